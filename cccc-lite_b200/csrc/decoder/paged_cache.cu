@@ -1,0 +1,332 @@
+// Keys and values into the pages of a cache and back, HBM-bound.  A group of lanes owns a row (a head of a token), sixteen elements
+// per lane: two 16-byte loads of BF16 become one 16-byte store of E4M3, and a page's rows of a head lie one behind the other, so
+// that a warp writes whole sectors wherever the tokens of a prompt follow each other.
+//
+// E4M3 rows carry a power of two: x / 2^k is exact, so the codes are rounded once, and what is read back is exact in BF16.
+#include "paged_attention.cuh"
+
+namespace b200
+{
+
+struct PagedRows
+{
+    PagedCache c;
+    PagedBatch b;
+    void* x[2];             // keys, values: [tokens][ld]
+    unsigned int ld[2];
+    unsigned int lanes[2];  // of a row, as a power of two; sixteen elements each
+    bool vec[2];            // eight elements in one access
+};
+
+template <class T>
+__device__ __forceinline__ void rows_load8(const T* src, unsigned int left, bool vec, float* x)
+{
+    if (vec && left >= 8)
+    {
+        const float4 a = load4(src), b = load4(src + 4);
+        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+        return;
+    }
+#pragma unroll
+    for (unsigned int j = 0; j < 8; j++) { x[j] = j < left ? Elem<T>::get(src[j]) : 0.f; }
+}
+template <>
+__device__ __forceinline__ void rows_load8(const __nv_bfloat16* src, unsigned int left, bool vec, float* x)
+{
+    if (vec && left >= 8)
+    {
+        const uint4 u = *reinterpret_cast<const uint4*>(src);
+        const uint32_t w[4] = { u.x, u.y, u.z, u.w };
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+        {
+            x[2 * j] = __uint_as_float(w[j] << 16);
+            x[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+        }
+        return;
+    }
+#pragma unroll
+    for (unsigned int j = 0; j < 8; j++) { x[j] = j < left ? __bfloat162float(src[j]) : 0.f; }
+}
+__device__ __forceinline__ void rows_store8(float* dst, unsigned int left, bool vec, const float* x)
+{
+    if (vec && left >= 8)
+    {
+        store4(dst, make_float4(x[0], x[1], x[2], x[3]));
+        store4(dst + 4, make_float4(x[4], x[5], x[6], x[7]));
+        return;
+    }
+#pragma unroll
+    for (unsigned int j = 0; j < 8; j++)
+    {
+        if (j < left) { dst[j] = x[j]; }
+    }
+}
+__device__ __forceinline__ void rows_store8(__nv_bfloat16* dst, unsigned int left, bool vec, const float* x)
+{
+    if (vec && left >= 8)
+    {
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+        {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * j], x[2 * j + 1]);
+            w[j] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+        *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+        return;
+    }
+#pragma unroll
+    for (unsigned int j = 0; j < 8; j++)
+    {
+        if (j < left) { dst[j] = __float2bfloat16_rn(x[j]); }
+    }
+}
+
+// Where a token of the batch lies in its sequence; its page, or -1.
+__device__ __forceinline__ int rows_place(const PagedRows& p, unsigned int token, unsigned int* at)
+{
+    const int e = p.b.token_entry[token];
+    if (e < (int)p.b.e0 || (unsigned int)e - p.b.e0 >= p.b.entries) { return -1; }
+    const int i = (int)token - p.b.start[e], pos = p.b.pos[e];
+    if (i < 0 || i >= p.b.n[e] || pos < 0) { return -1; }
+    const int slot = p.b.slot[e];
+    if ((unsigned int)slot >= p.c.slots) { return -1; }
+    *at = (unsigned int)pos + (unsigned int)i;
+    return paged_page(p.c, slot, *at);
+}
+
+// The exponent byte of a row whose largest finite element has these bits.  448 = 1.75 * 2^8.
+__device__ __forceinline__ unsigned int e4m3_exponent(uint32_t top)
+{
+    if (top == 0u) { return 127u; }
+    const int b = (int)(top >> 23) - 8 + ((top & 0x7FFFFFu) > 0x600000u ? 1 : 0);
+    return (unsigned int)max(b, 1);
+}
+// Four codes, the first one lowest.
+__device__ __forceinline__ uint32_t e4m3x4(const float* x)
+{
+    uint16_t a, b;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(a) : "f"(x[1]), "f"(x[0]));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(b) : "f"(x[3]), "f"(x[2]));
+    return (uint32_t)a | ((uint32_t)b << 16);
+}
+
+constexpr unsigned int PR_THREADS = 256;
+
+// blockIdx.y: keys, values
+template <class T, bool E4M3>
+__global__ void __launch_bounds__(PR_THREADS) pages_append_kernel(const __grid_constant__ PagedRows p)
+{
+    grid_dependency_launch();
+    grid_dependency_wait();
+    const unsigned int which = blockIdx.y, shift = p.lanes[which], width = which ? p.c.vdim : p.c.dim, ld = which ? p.c.v_ld : p.c.k_ld;
+    const unsigned int row = blockIdx.x * (PR_THREADS >> shift) + (threadIdx.x >> shift), d = (threadIdx.x & ((1u << shift) - 1u)) * 16;
+    if (row >= p.b.tokens * p.c.Hkv) { return; }    // rows are whole in a warp, and warps leave whole rows
+    const unsigned int token = p.b.t0 + row / p.c.Hkv, head = row % p.c.Hkv;
+    const T* src = (const T*)p.x[which] + (size_t)token * p.ld[which] + (size_t)head * width + d;
+    const unsigned int left = d < width ? width - d : 0;
+    float x[16];
+    rows_load8(src, left, p.vec[which], x);
+    rows_load8(src + 8, left > 8 ? left - 8 : 0, p.vec[which], x + 8);
+    unsigned int at = 0;
+    const int page = rows_place(p, token, &at);
+    const size_t to = page < 0 ? 0 : paged_row(p.c, page, head, at);
+    unsigned char* cache = which ? p.c.v : p.c.k;
+    if constexpr (E4M3)
+    {
+        uint32_t top = 0;
+#pragma unroll
+        for (int j = 0; j < 16; j++)
+        {
+            const uint32_t u = __float_as_uint(x[j]) & 0x7FFFFFFFu;
+            if (u < 0x7F800000u) { top = max(top, u); }
+        }
+        const unsigned int lanes = 1u << shift, mask = ((1u << lanes) - 1u) << (threadIdx.x & 31u & ~(lanes - 1u));
+        for (unsigned int o = lanes / 2; o > 0; o >>= 1) { top = max(top, __shfl_xor_sync(mask, top, o)); }
+        const unsigned int b = e4m3_exponent(top);
+        const float inv = paged_two(254u - b);
+#pragma unroll
+        for (int j = 0; j < 16; j++) { x[j] *= inv; }
+        if (page < 0) { return; }
+        if (d < ld) { *reinterpret_cast<uint4*>(cache + to * ld + d) = make_uint4(e4m3x4(x), e4m3x4(x + 4), e4m3x4(x + 8), e4m3x4(x + 12)); }
+        if (d == 0) { (which ? p.c.v_scale : p.c.k_scale)[to] = (unsigned char)b; }
+    }
+    else
+    {
+        if (page < 0 || d >= ld) { return; }
+        T* dst = (T*)cache + to * ld + d;
+        rows_store8(dst, 16, true, x);
+        rows_store8(dst + 8, 8, true, x + 8);
+    }
+}
+
+template <class T, bool E4M3>
+__global__ void __launch_bounds__(PR_THREADS) pages_read_kernel(const __grid_constant__ PagedRows p)
+{
+    grid_dependency_launch();
+    grid_dependency_wait();
+    const unsigned int which = blockIdx.y, shift = p.lanes[which], width = which ? p.c.vdim : p.c.dim, ld = which ? p.c.v_ld : p.c.k_ld;
+    const unsigned int row = blockIdx.x * (PR_THREADS >> shift) + (threadIdx.x >> shift), d = (threadIdx.x & ((1u << shift) - 1u)) * 16;
+    if (row >= p.b.tokens * p.c.Hkv || d >= width) { return; }
+    const unsigned int token = p.b.t0 + row / p.c.Hkv, head = row % p.c.Hkv;
+    unsigned int at = 0;
+    const int e = p.b.token_entry[token];
+    if (e < (int)p.b.e0 || (unsigned int)e - p.b.e0 >= p.b.entries || (int)token < p.b.start[e] || (int)token - p.b.start[e] >= p.b.n[e]) { return; }
+    const int page = rows_place(p, token, &at);
+    const unsigned char* cache = which ? p.c.v : p.c.k;
+    float x[16];
+    if (page < 0)
+    {
+#pragma unroll
+        for (int j = 0; j < 16; j++) { x[j] = 0.f; }
+    }
+    else
+    {
+        const size_t from = paged_row(p.c, page, head, at);
+        if constexpr (E4M3)
+        {
+            const uint4 u = *reinterpret_cast<const uint4*>(cache + from * ld + d);
+            const float two = paged_two((which ? p.c.v_scale : p.c.k_scale)[from]);
+            const uint32_t w[4] = { u.x, u.y, u.z, u.w };
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+            {
+                const uint32_t h = e4m3x2_to_f16x2(w[j / 2] >> (16 * (j % 2)));
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+                x[2 * j] = f.x * two;
+                x[2 * j + 1] = f.y * two;
+            }
+        }
+        else
+        {
+            const T* src = (const T*)cache + from * ld + d;
+            rows_load8(src, 8, true, x);
+            rows_load8(src + 8, 8, true, x + 8);
+        }
+    }
+    T* dst = (T*)p.x[which] + (size_t)token * p.ld[which] + (size_t)head * width + d;
+    rows_store8(dst, width - d, p.vec[which], x);
+    if (width - d > 8) { rows_store8(dst + 8, width - d - 8, p.vec[which], x + 8); }
+}
+
+}    // namespace b200
+
+using namespace b200;
+
+namespace b200
+{
+
+bool make_paged_cache(int dtype, const cuda_b200_pages* c, PagedCache* p)
+{
+    auto low = [](const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15u) != 0; };
+    if (!c || !c->k || !c->v || !c->table || low(c->k) || low(c->v) || (dtype != DT_BF16 && dtype != DT_FLOAT) || (c->type != dtype && c->type != DT_E4M3)) { return false; }
+    if (c->type == DT_E4M3 && (!c->k_scale || !c->v_scale || low(c->k_scale) || low(c->v_scale))) { return false; }
+    if (c->page < 16 || (c->page & (c->page - 1)) || c->Hkv == 0 || c->dim == 0 || c->vdim == 0 || c->dim > 256 || c->vdim > 256 || c->k_ld < c->dim
+        || c->v_ld < c->vdim || (c->k_ld % 16) || (c->v_ld % 16) || c->pages > 0x7FFFFFFFu || c->slots > 0x7FFFFFFFu
+        || (unsigned long long)c->ld_table * c->page > 0x40000000ull)
+    {
+        return false;
+    }
+    p->k = (unsigned char*)c->k;
+    p->v = (unsigned char*)c->v;
+    p->k_scale = (unsigned char*)c->k_scale;
+    p->v_scale = (unsigned char*)c->v_scale;
+    p->table = (const int*)c->table;
+    p->pages = c->pages;
+    p->shift = 0;
+    while ((1u << p->shift) < c->page) { p->shift++; }
+    p->slots = c->slots;
+    p->ld_table = c->ld_table;
+    p->Hkv = c->Hkv;
+    p->dim = c->dim;
+    p->vdim = c->vdim;
+    p->k_ld = c->k_ld;
+    p->v_ld = c->v_ld;
+    p->cap = c->ld_table * c->page;
+    return true;
+}
+
+bool make_paged_batch(const cuda_b200_batch* b, PagedBatch* p)
+{
+    if (!b->slot || !b->pos || !b->start || !b->n || b->first_token > 0x7FFFFFFFu - b->tokens || b->tokens > 0x7FFFFFFFu || b->entries > 0x7FFFFFFFu
+        || b->first_entry > 0x7FFFFFFFu - b->entries)
+    {
+        return false;
+    }
+    p->slot = (const int*)b->slot;
+    p->pos = (const int*)b->pos;
+    p->start = (const int*)b->start;
+    p->n = (const int*)b->n;
+    p->token_entry = (const int*)b->token_entry;
+    p->floor = (const int*)b->floor;
+    p->e0 = b->first_entry;
+    p->entries = b->entries;
+    p->t0 = b->first_token;
+    p->tokens = b->tokens;
+    p->max_n = b->max_n;
+    return true;
+}
+
+}    // namespace b200
+
+// The descriptors of a call that moves rows; the grid's size, or 0 where something is not taken.
+static unsigned int make_rows(int dtype, const cuda_b200_pages* c, void* k, unsigned int ldk, void* v, unsigned int ldv, const cuda_b200_batch* b, PagedRows* p)
+{
+    if (!k || !v || !b->token_entry || !make_paged_cache(dtype, c, &p->c) || !make_paged_batch(b, &p->b)) { return 0; }
+    if (ldk < (unsigned long long)c->Hkv * c->dim || ldv < (unsigned long long)c->Hkv * c->vdim) { return 0; }
+    const unsigned long long rows = (unsigned long long)b->tokens * c->Hkv;
+    if (rows > 0x7FFFFFFFull) { return 0; }
+    unsigned long long blocks = 0;
+    for (int i = 0; i < 2; i++)
+    {
+        const unsigned int width = i ? c->vdim : c->dim, ld = i ? ldv : ldk, row = i ? c->v_ld : c->k_ld;
+        p->x[i] = i ? v : k;
+        p->ld[i] = ld;
+        p->vec[i] = (width % 8) == 0 && (ld % 8) == 0 && (reinterpret_cast<uintptr_t>(p->x[i]) % 16) == 0;
+        // padding behind the 256 elements that a row may have stays as it is: it is never read
+        p->lanes[i] = 0;
+        while ((16u << p->lanes[i]) < row && p->lanes[i] < 4) { p->lanes[i]++; }
+        const unsigned long long per = PR_THREADS >> p->lanes[i], n = (rows + per - 1) / per;
+        if (n > blocks) { blocks = n; }
+    }
+    return (unsigned int)blocks;
+}
+
+C_EXPORT int cuda_b200_pages_append(int dtype, const cuda_b200_pages* c, const void* k, unsigned int ldk, const void* v, unsigned int ldv,
+    const cuda_b200_batch* b, void* stream, unsigned int flags)
+{
+    if (!b) { return -1; }
+    if (b->tokens == 0 || b->entries == 0) { return 0; }
+    PagedRows p;
+    const unsigned int blocks = make_rows(dtype, c, const_cast<void*>(k), ldk, const_cast<void*>(v), ldv, b, &p);
+    if (blocks == 0) { return -1; }
+    const bool pdl = (flags & 1u) != 0, coded = c->type == DT_E4M3;
+    const dim3 grid(blocks, 2), block(PR_THREADS);
+    if (dtype == DT_BF16)
+    {
+        return coded ? launch_kernel("pages_append", pages_append_kernel<__nv_bfloat16, true>, grid, block, 0, stream, pdl, p)
+                     : launch_kernel("pages_append", pages_append_kernel<__nv_bfloat16, false>, grid, block, 0, stream, pdl, p);
+    }
+    return coded ? launch_kernel("pages_append", pages_append_kernel<float, true>, grid, block, 0, stream, pdl, p)
+                 : launch_kernel("pages_append", pages_append_kernel<float, false>, grid, block, 0, stream, pdl, p);
+}
+
+C_EXPORT int cuda_b200_pages_read(int dtype, const cuda_b200_pages* c, void* k, unsigned int ldk, void* v, unsigned int ldv, const cuda_b200_batch* b,
+    void* stream, unsigned int flags)
+{
+    if (!b) { return -1; }
+    if (b->tokens == 0 || b->entries == 0) { return 0; }
+    PagedRows p;
+    const unsigned int blocks = make_rows(dtype, c, k, ldk, v, ldv, b, &p);
+    if (blocks == 0) { return -1; }
+    const bool pdl = (flags & 1u) != 0, coded = c->type == DT_E4M3;
+    const dim3 grid(blocks, 2), block(PR_THREADS);
+    if (dtype == DT_BF16)
+    {
+        return coded ? launch_kernel("pages_read", pages_read_kernel<__nv_bfloat16, true>, grid, block, 0, stream, pdl, p)
+                     : launch_kernel("pages_read", pages_read_kernel<__nv_bfloat16, false>, grid, block, 0, stream, pdl, p);
+    }
+    return coded ? launch_kernel("pages_read", pages_read_kernel<float, true>, grid, block, 0, stream, pdl, p)
+                 : launch_kernel("pages_read", pages_read_kernel<float, false>, grid, block, 0, stream, pdl, p);
+}

@@ -29,6 +29,14 @@ Batch = _struct("Batch", ("slot", "pos", "start", "n", "token_entry", "floor"), 
 Attention = _struct("Attention", ("qkvg", "out", "k_cache", "v_cache", "v_first", "work", "q_norm", "k_norm", "rotary", "sink", "head_gate"),
                     ("ld", "ldo", "k_off", "v_off", "g_off", "v_first_ld", "H", "Hkv", "dim", "vdim", "k_ld", "v_ld", "T_max", "slots", "q_ld", "rot_dims", "ld_gate",
                      "window"), ("v_mix", "qk_norm", "gate", "rot_interleaved", "no_append"), ("mix", "eps", "scale"))
+Pages = _struct("Pages", ("k", "v", "k_scale", "v_scale", "table"), ("pages", "page", "slots", "ld_table", "Hkv", "dim", "vdim", "k_ld", "v_ld"), ("type",))
+
+
+class PagedAttention(C.Structure):
+    _fields_ = [(n, _vp) for n in ("q", "out", "work", "sink")] + [("work_bytes", C.c_ulonglong)] + [(n, _u) for n in ("ldq", "ldo", "H", "window", "first")] + [
+        ("scale", _f)]
+
+
 Latent = _struct("Latent", ("down", "cq", "cache", "q_norm", "kv_norm", "rotary"), ("ld", "ld_cq", "kv_off", "q_rank", "kv_rank", "rot_dim", "c_ld", "T_max"), (),
                  ("eps",))
 Expand = _struct("Expand", ("cache", "c", "K", "floor", "pos2"), ("c_ld", "T_max", "kv_rank", "rot_dim", "ld_c", "k_ld", "T", "dim", "heads", "max_rows"))
@@ -43,6 +51,10 @@ SYMBOLS = {
     "cuda_b200_linear_rows": (_i, [_i, _u, C.POINTER(Linear), _vp, _u, _i]),
     "cuda_b200_attention_work_bytes": (C.c_ulonglong, [_u]),
     "cuda_b200_attention_rows": (_i, [_i, C.POINTER(Attention), C.POINTER(Batch), _vp, _u, _i]),
+    "cuda_b200_pages_append": (_i, [_i, C.POINTER(Pages), _vp, _u, _vp, _u, C.POINTER(Batch), _vp, _u]),
+    "cuda_b200_pages_read": (_i, [_i, C.POINTER(Pages), _vp, _u, _vp, _u, C.POINTER(Batch), _vp, _u]),
+    "cuda_b200_paged_attention_work_bytes": (C.c_ulonglong, [_u, _u, _u, _u]),
+    "cuda_b200_paged_attention_rows": (_i, [_i, C.POINTER(PagedAttention), C.POINTER(Pages), C.POINTER(Batch), _vp, _u, _i]),
     "cuda_b200_rotary_table": (_i, [_vp, _u, _u, C.c_double, _vp]),
     "cuda_b200_latent_down": (_i, [_i, C.POINTER(Latent), C.POINTER(Batch), _vp, _u]),
     "cuda_b200_latent_query": (_i, [_i, _vp, _u, _u, _u, _vp, _u, _u, _u, _u, _u, _vp, _u, C.POINTER(Batch), _vp, _u]),
@@ -110,6 +122,22 @@ def attention(dtype, desc, batch, flags=0, kernel=0):
 
 def attention_work_bytes(vdim):
     return int(lib().cuda_b200_attention_work_bytes(vdim))
+
+
+def pages_append(dtype, pages, k, ldk, v, ldv, batch, flags=0):
+    return lib().cuda_b200_pages_append(dtype, C.byref(pages), _ptr(k), ldk, _ptr(v), ldv, C.byref(batch), raw_stream(), flags)
+
+
+def pages_read(dtype, pages, k, ldk, v, ldv, batch, flags=0):
+    return lib().cuda_b200_pages_read(dtype, C.byref(pages), _ptr(k), ldk, _ptr(v), ldv, C.byref(batch), raw_stream(), flags)
+
+
+def paged_attention_work_bytes(H, Hkv, vdim, max_n):
+    return int(lib().cuda_b200_paged_attention_work_bytes(H, Hkv, vdim, max_n))
+
+
+def paged_attention(dtype, desc, pages, batch, flags=0, kernel=0):
+    return lib().cuda_b200_paged_attention_rows(dtype, C.byref(desc), C.byref(pages), C.byref(batch), raw_stream(), flags, kernel)
 
 
 def rotary_table(table, rows, dims, base):

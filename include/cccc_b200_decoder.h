@@ -144,6 +144,54 @@ C_EXPORT unsigned long long cuda_b200_attention_work_bytes(unsigned int vdim);
 C_EXPORT int cuda_b200_attention_rows(int dtype, const cuda_b200_attention* a, const cuda_b200_batch* b, void* stream, unsigned int flags,
     int kernel);
 
+/* A cache in pages: a sequence's positions i * page .. (i + 1) * page - 1 lie on the page that its table row names at i.  An
+ * entry outside 0 .. pages - 1, like a place behind the table's row or a slot outside 0 .. slots - 1, is no page: nothing is
+ * written there, it reads as zeros, and attention does not see its keys.  Sequences may share pages that are only read.
+ * Caches are held in the call's dtype, or (type 4) in E4M3 with an exponent byte per row and head: a row stands for its codes
+ * times 2^(b - 127), b in 1 .. 254.  Rows have k_ld / v_ld elements (multiples of 16); dim and vdim go up to 256.  k and v are
+ * 16-byte aligned, and so are the scales. */
+typedef struct cuda_b200_pages
+{
+    void* k;                   /* [pages][Hkv][page][k_ld] */
+    void* v;                   /* [pages][Hkv][page][v_ld] */
+    void* k_scale;             /* E4M3: bytes [pages][Hkv][page] */
+    void* v_scale;
+    const void* table;         /* int32 [slots][ld_table] */
+    unsigned int pages, page;  /* page: rows of a page, a power of two from 16 on */
+    unsigned int slots, ld_table;
+    unsigned int Hkv, dim, vdim, k_ld, v_ld;
+    int type;
+} cuda_b200_pages;
+/* Writes the batch's keys and values, [tokens][ldk] with a head every dim and [tokens][ldv] with a head every vdim, at their
+ * positions; the padding of the rows becomes zero.  E4M3: a row's power of two is the smallest one, from 2^-126 on, with which
+ * its largest finite element is at most 448 (1 for a row of zeros); codes are rounded to nearest, ties to even, infinities become
+ * the largest code of their sign, NaN stays NaN.  No two tokens of a call may go to one place. */
+C_EXPORT int cuda_b200_pages_append(int dtype, const cuda_b200_pages* c, const void* k, unsigned int ldk, const void* v, unsigned int ldv,
+    const cuda_b200_batch* b, void* stream, unsigned int flags);
+/* The inverse: the rows at positions pos[e] .. pos[e] + n[e] - 1 of the entries' sequences, as dtype, to rows start[e] .. of k and v. */
+C_EXPORT int cuda_b200_pages_read(int dtype, const cuda_b200_pages* c, void* k, unsigned int ldk, void* v, unsigned int ldv,
+    const cuda_b200_batch* b, void* stream, unsigned int flags);
+
+/* Softmax attention of the batch's queries over a paged cache that holds their keys and values already (query head h reads kv
+ * head h / (H / Hkv)).  The token at position t sees the keys floor .. t (floor: the entry's, or 0), with a window those above t -
+ * window and the `first` keys from floor on.  A row that sees no key, or whose scores are all minus infinity, gives zeros.  Keys
+ * and values that no row of the entry sees may hold anything; one that is no number may reach every row of its entry in the call. */
+typedef struct cuda_b200_paged_attention
+{
+    const void* q;             /* [tokens][ldq] dtype: a head every dim */
+    void* out;                 /* [tokens][ldo] dtype: a head every vdim */
+    void* work;                /* scratch of cuda_b200_paged_attention_work_bytes, 16-byte aligned; for one call at a time */
+    const void* sink;          /* float [H]: a score that takes part in the softmax denominator only; or NULL */
+    unsigned long long work_bytes;
+    unsigned int ldq, ldo, H, window, first;
+    float scale;
+} cuda_b200_paged_attention;
+/* Bytes of scratch on the current device for calls of up to max_n tokens per entry (0 for sizes that are not taken). */
+C_EXPORT unsigned long long cuda_b200_paged_attention_work_bytes(unsigned int H, unsigned int Hkv, unsigned int vdim, unsigned int max_n);
+/* kernel: 0 = by shape, 1 = the plain kernel (always in float mode). */
+C_EXPORT int cuda_b200_paged_attention_rows(int dtype, const cuda_b200_paged_attention* a, const cuda_b200_pages* c, const cuda_b200_batch* b, void* stream,
+    unsigned int flags, int kernel);
+
 /* Latent attention keeps per token one row [latent | rotated key part] for all heads.
  * _down: for every token of the batch, query latent cq = rms_norm(down[0 .. q_rank)) * q_norm, and the cache row
  * [rms_norm(down[kv_off .. + kv_rank)) * kv_norm | rotated down[kv_off + kv_rank .. + rot_dim)]; pairs are 2i and 2i + 1.
