@@ -8,7 +8,7 @@ namespace b200
 // ---- plain kernel ------------------------------------------------------------------------------------------------
 // Four packed query rows per segment, units of 32 keys, one key per lane for the scores and one element per lane for the values.
 // The warps of a CTA take the units in turn, each with its own maximum and sum.
-constexpr unsigned int PP_UNIT = 32, PP_ROWS = 4, PP_WARPS = 4, PP_THREADS = 32 * PP_WARPS, PP_ELEMS = 8;    // elements of a value row per lane
+constexpr unsigned int PP_UNIT = 32, PP_ROWS = kPagedPlainRows, PP_WARPS = 4, PP_THREADS = 32 * PP_WARPS, PP_ELEMS = 8;    // elements of a value row per lane
 
 template <class C>
 __device__ __forceinline__ float4 cache4(const C* p) { return load4(p); }
@@ -249,8 +249,7 @@ static int combine(const PagedParams& p, unsigned int rows, unsigned int ctas, c
 
 // ---- dispatch ----------------------------------------------------------------------------------------------------
 // Scratch: a header for each CTA of the kernel that has most of them, then the pieces.
-constexpr unsigned int kPlainCtas = 4;    // per SM
-static size_t header_bytes(unsigned int sms) { return (size_t)sms * kPlainCtas * sizeof(PagedHeader); }
+static size_t header_bytes(unsigned int sms) { return (size_t)sms * kPagedPlainCtas * sizeof(PagedHeader); }
 static size_t work_of(unsigned int sms, unsigned int ctas_per_sm, unsigned int rows, unsigned int vdim)
 {
     return header_bytes(sms) + 2 * (size_t)sms * ctas_per_sm * paged_piece(rows, vdim) * 4;
@@ -272,7 +271,9 @@ C_EXPORT unsigned long long cuda_b200_paged_attention_work_bytes(unsigned int H,
 {
     const DecoderDevice* dev = decoder_device();
     if (!dev || Hkv == 0 || H == 0 || (H % Hkv) || vdim == 0 || vdim > 256 || (unsigned long long)max_n * (H / Hkv) > 0x7FFFFFFFull) { return 0; }
-    return work_of(dev->sm_count, kPlainCtas, PP_ROWS, vdim);
+    // the plain kernel and the one for few rows take the same
+    static_assert(kPagedPlainCtas * kPagedPlainRows == kPagedRowsRows, "");
+    return work_of(dev->sm_count, 1, kPagedRowsRows, vdim);
 }
 
 C_EXPORT int cuda_b200_paged_attention_rows(int dtype, const cuda_b200_paged_attention* a, const cuda_b200_pages* c, const cuda_b200_batch* b, void* stream,
@@ -283,7 +284,7 @@ C_EXPORT int cuda_b200_paged_attention_rows(int dtype, const cuda_b200_paged_att
     PagedParams p;
     if (!a->q || !a->out || !a->work || !make_paged_cache(dtype, c, &p.c) || !make_paged_batch(b, &p.b)) { return -1; }
     if (a->H == 0 || (a->H % c->Hkv) || a->ldq < (unsigned long long)a->H * c->dim || a->ldo < (unsigned long long)a->H * c->vdim
-        || (unsigned long long)b->max_n * (a->H / c->Hkv) > 0x7FFFFFFFull || (reinterpret_cast<uintptr_t>(a->work) & 15u) || kernel < 0 || kernel > 1)
+        || (unsigned long long)b->max_n * (a->H / c->Hkv) > 0x7FFFFFFFull || (reinterpret_cast<uintptr_t>(a->work) & 15u) || kernel < 0 || kernel > 2)
     {
         return -1;
     }
@@ -304,8 +305,15 @@ C_EXPORT int cuda_b200_paged_attention_rows(int dtype, const cuda_b200_paged_att
     const bool pdl = (flags & 1u) != 0, coded = c->type == DT_E4M3;
     const cudaStream_t st = (cudaStream_t)stream;
     const unsigned int rows = b->max_n * p.G, sms = (unsigned int)dev->sm_count;
-    if (a->work_bytes < work_of(sms, kPlainCtas, PP_ROWS, c->vdim)) { return -1; }
-    const unsigned int ctas = sms * kPlainCtas;
+    if (a->work_bytes < work_of(sms, 1, kPagedRowsRows, c->vdim)) { return -1; }
+    if (dtype == DT_FLOAT) { kernel = 1; }
+    if (kernel == 0) { kernel = 2; }
+    if (kernel == 2)
+    {
+        const int rc = launch_paged_rows(p, coded, sms, st, pdl);
+        return rc ? rc : combine<__nv_bfloat16, kPagedRowsRows>(p, rows < kPagedRowsRows ? rows : kPagedRowsRows, sms, st);
+    }
+    const unsigned int ctas = sms * kPagedPlainCtas;
     if (dtype == DT_FLOAT) { return coded ? run_plain<float, unsigned char>(p, rows, ctas, st, pdl) : run_plain<float, float>(p, rows, ctas, st, pdl); }
     return coded ? run_plain<__nv_bfloat16, unsigned char>(p, rows, ctas, st, pdl) : run_plain<__nv_bfloat16, __nv_bfloat16>(p, rows, ctas, st, pdl);
 }

@@ -7,7 +7,7 @@ from __graft_entry__ import load_package
 
 pytestmark = pytest.mark.gpu
 FLOAT, BF16, E4M3 = 0, 3, 4
-PLAIN = 1
+PLAIN, FEW = 1, 2
 
 
 @pytest.fixture(scope="module")
@@ -321,7 +321,7 @@ BATCHES = [
 
 
 def kinds(dtype, H, Hkv, entries):
-    return [PLAIN] if dtype == FLOAT else [0, PLAIN]
+    return [PLAIN] if dtype == FLOAT else [0, PLAIN, FEW]
 
 
 @pytest.mark.parametrize("dtype,type_", TYPES)
