@@ -19,7 +19,9 @@ enum : unsigned int
     WAIT_ATTENTION_TILE = 2,
     WAIT_MLSTM_STATES = 3,
     WAIT_MLSTM_OUTPUTS = 4,
-    WAIT_ATTENTION_LATENT = 5
+    WAIT_ATTENTION_LATENT = 5,
+    WAIT_PAGED_ROWS = 6,
+    WAIT_PAGED_TILE = 7
 };
 __device__ __forceinline__ void note_timeout(unsigned int* status, unsigned int kernel, unsigned int role, unsigned int step)
 {

@@ -31,6 +31,11 @@ __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two)
     asm("{\n\t.reg .b16 lo;\n\tcvt.u16.u32 lo, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(two));
     return r;
 }
+// Four codes: the lower two, the upper two.
+__device__ __forceinline__ void e4m3x4_to_f16x2(uint32_t four, uint32_t& a, uint32_t& b)
+{
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\tcvt.rn.f16x2.e4m3x2 %1, hi;\n\t}" : "=r"(a), "=r"(b) : "r"(four));
+}
 __device__ __forceinline__ float paged_exp2(float x)
 {
     float y;

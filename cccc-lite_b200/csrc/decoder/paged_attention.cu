@@ -310,8 +310,9 @@ C_EXPORT int cuda_b200_paged_attention_rows(int dtype, const cuda_b200_paged_att
     if (kernel == 0) { kernel = 2; }
     if (kernel == 2)
     {
-        const int rc = launch_paged_rows(p, coded, sms, st, pdl);
-        return rc ? rc : combine<__nv_bfloat16, kPagedRowsRows>(p, rows < kPagedRowsRows ? rows : kPagedRowsRows, sms, st);
+        const int rc = launch_paged_rows(p, coded, rows, sms, st, pdl);
+        if (rc) { return rc; }
+        return rows <= 8 ? combine<__nv_bfloat16, 8>(p, rows, sms, st) : combine<__nv_bfloat16, kPagedRowsRows>(p, rows < kPagedRowsRows ? rows : kPagedRowsRows, sms, st);
     }
     const unsigned int ctas = sms * kPagedPlainCtas;
     if (dtype == DT_FLOAT) { return coded ? run_plain<float, unsigned char>(p, rows, ctas, st, pdl) : run_plain<float, float>(p, rows, ctas, st, pdl); }

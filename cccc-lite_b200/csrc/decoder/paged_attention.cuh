@@ -1,6 +1,7 @@
 // Attention over a cache in pages: the host side that its kernels share.
 #pragma once
 
+#include "../tensor_map.cuh"
 #include "paged.cuh"
 
 namespace b200
@@ -10,10 +11,24 @@ namespace b200
 bool make_paged_cache(int dtype, const cuda_b200_pages* c, PagedCache* p);
 bool make_paged_batch(const cuda_b200_batch* b, PagedBatch* p);
 
+// A cache's rows as [pages][Hkv * page][ld], copied `rows` at a time in pieces of `cols` elements.
+inline bool make_paged_map(CUtensorMap* map, bool coded, const void* base, unsigned int ld, const PagedCache& c, unsigned int cols, unsigned int rows, bool swizzle)
+{
+    EncodeTiledFn fn = encode_tiled_fn();
+    if (!fn || c.pages == 0) { return false; }
+    const cuuint64_t bytes = (cuuint64_t)ld * (coded ? 1 : 2), of_page = (cuuint64_t)c.Hkv << c.shift;
+    const cuuint64_t dims[3] = { ld, of_page, c.pages }, strides[2] = { bytes, bytes * of_page };
+    const cuuint32_t box[3] = { cols, rows, 1 }, one[3] = { 1, 1, 1 };
+    return fn(map, coded ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, one,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE)
+        == CUDA_SUCCESS;
+}
+
 // The kernels' segments: packed query rows, CTAs per SM.
-constexpr unsigned int kPagedPlainRows = 4, kPagedPlainCtas = 4, kPagedRowsRows = 16;
+constexpr unsigned int kPagedPlainRows = 4, kPagedPlainCtas = 4, kPagedRowsRows = 16;    // (8 where no entry has more)
 
 // paged_rows.cu: `ctas` CTAs at most, one per SM
-int launch_paged_rows(PagedParams& p, bool coded, unsigned int ctas, cudaStream_t stream, bool pdl);
+int launch_paged_rows(PagedParams& p, bool coded, unsigned int rows, unsigned int ctas, cudaStream_t stream, bool pdl);
 
 }    // namespace b200

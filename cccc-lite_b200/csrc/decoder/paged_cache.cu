@@ -223,8 +223,8 @@ bool make_paged_cache(int dtype, const cuda_b200_pages* c, PagedCache* p)
     if (!c || !c->k || !c->v || !c->table || low(c->k) || low(c->v) || (dtype != DT_BF16 && dtype != DT_FLOAT) || (c->type != dtype && c->type != DT_E4M3)) { return false; }
     if (c->type == DT_E4M3 && (!c->k_scale || !c->v_scale || low(c->k_scale) || low(c->v_scale))) { return false; }
     if (c->page < 16 || (c->page & (c->page - 1)) || c->Hkv == 0 || c->dim == 0 || c->vdim == 0 || c->dim > 256 || c->vdim > 256 || c->k_ld < c->dim
-        || c->v_ld < c->vdim || (c->k_ld % 16) || (c->v_ld % 16) || c->pages > 0x7FFFFFFFu || c->slots > 0x7FFFFFFFu
-        || (unsigned long long)c->ld_table * c->page > 0x40000000ull)
+        || c->v_ld < c->vdim || (c->k_ld % 16) || (c->v_ld % 16) || c->pages == 0 || c->pages > 0x7FFFFFFFu || c->slots > 0x7FFFFFFFu
+        || (unsigned long long)c->ld_table * c->page > 0x40000000ull || (unsigned long long)c->Hkv * c->page > 0x40000000ull)
     {
         return false;
     }

@@ -182,7 +182,7 @@ def _calls():
 
 BAD_PAGES = [dict(k=None), dict(v=None), dict(table=None), dict(k=0x10008), dict(v=0x10001), dict(page=8), dict(page=24), dict(page=0), dict(Hkv=0), dict(dim=0),
              dict(vdim=0), dict(dim=257, k_ld=272), dict(vdim=257, v_ld=272), dict(k_ld=48), dict(v_ld=72), dict(k_ld=63), dict(type=0), dict(type=5),
-             dict(k_scale=None), dict(v_scale=None), dict(k_scale=0x10004), dict(v_scale=0x10002), dict(ld_table=1 << 27)]
+             dict(k_scale=None), dict(v_scale=None), dict(k_scale=0x10004), dict(v_scale=0x10002), dict(ld_table=1 << 27), dict(pages=0), dict(pages=1 << 31), dict(page=1 << 30, ld_table=0)]
 
 
 @pytest.mark.parametrize("bad", BAD_PAGES, ids=str)
