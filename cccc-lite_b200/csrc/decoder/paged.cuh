@@ -13,7 +13,7 @@ struct PagedParams : PagedPlan
     void* out;
     const float* sink;
     PagedHeader* header;    // per CTA
-    float* partial;         // per CTA two pieces: one of a segment begun before, one of the segment left unfinished
+    float* partial;         // per worker two pieces: one of a segment begun before, one of the segment left unfinished
     unsigned int ldq, ldo, H;
     float scale;
 };
@@ -43,9 +43,15 @@ __device__ __forceinline__ float paged_exp2(float x)
     return y;
 }
 
-// All of the CTA's THREADS threads; `warps` is shared memory for THREADS / 32 sums, `share` is shared too.
+// Where the units of the entries lie, in shared memory: before[i] units come before those of thread i's entries, before[THREADS] are all.
+template <unsigned int THREADS>
+struct PagedSums
+{
+    unsigned long long before[THREADS + 1], warps[THREADS / 32];
+};
+// By all of the CTA's THREADS threads.
 template <unsigned int UNIT, unsigned int ROWS, unsigned int THREADS>
-__device__ __forceinline__ void paged_share(const PagedParams& p, unsigned long long* warps, PagedShare* share)
+__device__ __forceinline__ void paged_sums(const PagedParams& p, PagedSums<THREADS>* s)
 {
     const unsigned int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const unsigned int per = (p.b.entries + THREADS - 1) / THREADS, e_begin = threadIdx.x * per, e_end = min(e_begin + per, p.b.entries);
@@ -58,27 +64,35 @@ __device__ __forceinline__ void paged_share(const PagedParams& p, unsigned long 
         const unsigned long long x = __shfl_up_sync(0xFFFFFFFFu, sum, o);
         if (lane >= (unsigned int)o) { sum += x; }
     }
-    if (lane == 31) { warps[warp] = sum; }
+    if (lane == 31) { s->warps[warp] = sum; }
     __syncthreads();
-    unsigned long long before = 0, total = 0;
+    unsigned long long before = 0;
 #pragma unroll
-    for (unsigned int w = 0; w < THREADS / 32; w++)
-    {
-        if (w < warp) { before += warps[w]; }
-        total += warps[w];
-    }
-    before += sum - mine;
-    const unsigned int ctas = paged_ctas(total, p.least, gridDim.x);
-    const unsigned long long begin = paged_begin(total, blockIdx.x, ctas), end = paged_begin(total, blockIdx.x + 1, ctas);
-    if (threadIdx.x == 0)
-    {
-        share->total = total;
-        share->begin = begin;
-        share->end = end;
-        share->ctas = ctas;
-    }
-    if (begin >= before && begin < before + mine && begin < end) { paged_find<UNIT, ROWS>(p, p.b.e0 + e_begin, p.b.e0 + e_end, begin - before, share); }
+    for (unsigned int w = 0; w < THREADS / 32; w++) { before += w < warp ? s->warps[w] : 0; }
+    s->before[threadIdx.x] = before + sum - mine;
+    if (threadIdx.x == THREADS - 1) { s->before[THREADS] = before + sum; }
     __syncthreads();
+}
+// The share of one of `most` workers; by any thread, after paged_sums.
+template <unsigned int UNIT, unsigned int ROWS, unsigned int THREADS>
+__device__ __forceinline__ PagedShare paged_share(const PagedParams& p, const PagedSums<THREADS>& s, unsigned int worker, unsigned int most)
+{
+    PagedShare x = {};
+    x.total = s.before[THREADS];
+    x.workers = paged_workers(x.total, p.least, most);
+    x.begin = paged_begin(x.total, worker, x.workers);
+    x.end = paged_begin(x.total, worker + 1, x.workers);
+    if (x.begin >= x.end) { return x; }
+    unsigned int lo = 0, hi = THREADS;    // before[lo] <= begin < before[hi]
+    while (hi - lo > 1)
+    {
+        const unsigned int mid = (lo + hi) / 2;
+        if (s.before[mid] <= x.begin) { lo = mid; }
+        else { hi = mid; }
+    }
+    const unsigned int per = (p.b.entries + THREADS - 1) / THREADS;
+    paged_find<UNIT, ROWS>(p, p.b.e0 + lo * per, p.b.e0 + min((lo + 1) * per, p.b.entries), x.begin - s.before[lo], &x);
+    return x;
 }
 
 template <class T>
@@ -102,6 +116,80 @@ __device__ __forceinline__ float paged_factor(const PagedParams& p, unsigned int
     if (m == -INFINITY && l == 0.f) { return 0.f; }
     if (p.sink != nullptr) { l += paged_exp2(fmaf(p.sink[head], 1.44269504088896341f, -m)); }
     return 1.0f / l;
+}
+
+// A warp puts four neighbouring rows of pieces together, eight lanes a row: lane s of them has the elements 32 k + 4 s .. of k < K.
+template <int K>
+struct PagedQuad
+{
+    float top, sum;
+    float4 acc[K];
+};
+// Rows r .. r + 3 (those below `end`) of `n` pieces, up to eight, in their order: the first one, then those at `others`, `step` floats from
+// one to the next.  Everything that is asked for is under way at once.
+template <int K>
+__device__ __forceinline__ PagedQuad<K> paged_join(const float* first, const float* others, size_t step, unsigned int n, unsigned int r, unsigned int end, unsigned int VL,
+    unsigned int rows)
+{
+    const unsigned int lane = threadIdx.x & 31, s = lane & 7u, row = r + (lane >> 3);
+    const bool real = row < end;
+    auto at = [&](unsigned int j) { return j == 0 ? first : others + (size_t)(j - 1) * step; };
+    const float m = real && s < n ? at(s)[rows * VL + row] : -INFINITY, l = real && s < n ? at(s)[rows * VL + rows + row] : 0.f;
+    constexpr unsigned int B = K <= 4 ? 4 : 2;    // pieces at a time
+    float4 y[B][K];
+    auto fetch = [&](unsigned int j0) {
+#pragma unroll
+        for (unsigned int j = 0; j < B; j++)
+        {
+#pragma unroll
+            for (unsigned int k = 0; k < K; k++)
+            {
+                y[j][k] = real && j0 + j < n && k * 32 + s * 4 < VL ? load4(at(j0 + j) + (size_t)row * VL + k * 32 + s * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+        }
+    };
+    fetch(0);
+    PagedQuad<K> x;
+    x.top = m;
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) { x.top = fmaxf(x.top, __shfl_xor_sync(0xFFFFFFFFu, x.top, o)); }
+    const float f = s >= n ? 0.f : x.top == -INFINITY ? 1.f : exp2f(m - x.top);
+    x.sum = f * l;
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) { x.sum += __shfl_xor_sync(0xFFFFFFFFu, x.sum, o); }
+#pragma unroll
+    for (unsigned int k = 0; k < K; k++) { x.acc[k] = make_float4(0.f, 0.f, 0.f, 0.f); }
+    for (unsigned int j0 = 0; j0 < n; j0 += B)
+    {
+        if (j0 != 0) { fetch(j0); }
+#pragma unroll
+        for (unsigned int j = 0; j < B; j++)
+        {
+            const float w = __shfl_sync(0xFFFFFFFFu, f, (lane & 24u) + ((j0 + j) & 7u));
+#pragma unroll
+            for (unsigned int k = 0; k < K; k++)
+            {
+                x.acc[k] = make_float4(fmaf(w, y[j][k].x, x.acc[k].x), fmaf(w, y[j][k].y, x.acc[k].y), fmaf(w, y[j][k].z, x.acc[k].z), fmaf(w, y[j][k].w, x.acc[k].w));
+            }
+        }
+    }
+    return x;
+}
+// Row r + lane / 8 of a segment (its packed row `row`, of those below `end`) as an output.
+template <class T, int K>
+__device__ __forceinline__ void paged_put(const PagedParams& p, const PagedQuad<K>& x, unsigned int start, unsigned int kvh, unsigned int row, bool real)
+{
+    if (!real) { return; }
+    const unsigned int s = threadIdx.x & 7u, head = kvh * p.G + row % p.G;
+    const float f = paged_factor(p, head, x.top, x.sum);
+    const bool vec = paged_vec4<T>(p);
+    T* out = (T*)p.out + (size_t)(start + row / p.G) * p.ldo + (size_t)head * p.c.vdim;
+#pragma unroll
+    for (unsigned int k = 0; k < K; k++)
+    {
+        const unsigned int d = k * 32 + s * 4;
+        if (d < p.c.vdim) { paged_store4(out, d, p.c.vdim, vec, make_float4(x.acc[k].x * f, x.acc[k].y * f, x.acc[k].z * f, x.acc[k].w * f)); }
+    }
 }
 
 }    // namespace b200

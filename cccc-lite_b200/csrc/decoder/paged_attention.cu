@@ -31,15 +31,15 @@ template <class T, class C>
 __global__ void __launch_bounds__(PP_THREADS) paged_plain_kernel(const __grid_constant__ PagedParams p)
 {
     constexpr bool CODED = sizeof(C) == 1;
-    __shared__ PagedShare share;
-    __shared__ unsigned long long sums[PP_WARPS];
+    __shared__ PagedSums<PP_THREADS> sums;
     __shared__ __align__(16) float q[PP_ROWS][256];
     __shared__ float acc_s[PP_WARPS][PP_ROWS][32 * PP_ELEMS];
     __shared__ float max_s[PP_WARPS][PP_ROWS], sum_s[PP_WARPS][PP_ROWS];
     const unsigned int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     grid_dependency_launch();
     grid_dependency_wait();
-    paged_share<PP_UNIT, PP_ROWS, PP_THREADS>(p, sums, &share);
+    paged_sums<PP_UNIT, PP_ROWS, PP_THREADS>(p, &sums);
+    const PagedShare share = paged_share<PP_UNIT, PP_ROWS, PP_THREADS>(p, sums, blockIdx.x, gridDim.x);
     PagedHeader header = {};
     PagedCursor<PP_UNIT, PP_ROWS> cur;
     unsigned long long at = share.begin;
@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(PP_THREADS) paged_plain_kernel(const __grid_co
             }
         }
         __syncthreads();
-        if (!whole && cur.unit == 0) { header = cur.header(share, at, blockIdx.x); }
+        if (!whole && cur.unit == 0) { header = PagedHeader{ cur.last(share, at) - blockIdx.x + 1, blockIdx.x, s.rows, s.r0, cur.v.start, cur.kvh }; }
         at += units;
         if (at < share.end) { cur.next(p); }
     }
@@ -189,70 +189,108 @@ __global__ void __launch_bounds__(PP_THREADS) paged_plain_kernel(const __grid_co
 }
 
 // ---- pieces together ---------------------------------------------------------------------------------------------
-// A warp per row: the segment that CTA x left unfinished, its own piece and the first ones of the CTAs behind it.
-template <class T, unsigned int ROWS>
-__global__ void __launch_bounds__(128) paged_combine_kernel(const __grid_constant__ PagedParams p)
+// The segments that CTAs left unfinished: the piece of the worker that has begun it, then the first pieces of the CTAs behind it, in their
+// order.  A task is four rows of such a segment, rows 4 i .. of CTA w's the task of CTA (w + i) % gridDim.x, so that few segments still reach
+// many CTAs.  A task's pieces are dealt to a team of warps (a sequence alone comes in a piece from every CTA), whose parts meet in
+// shared memory, again in order.  Small enough to wait beside the kernel before it on an SM.
+constexpr unsigned int PC_WARPS = 4, PC_THREADS = 32 * PC_WARPS;
+
+// K: 32 elements of values each; per: workers of a CTA; piece_rows: rows that a piece has room for
+template <class T, int K>
+__global__ void __launch_bounds__(PC_THREADS, 4) paged_combine_kernel(const __grid_constant__ PagedParams p, unsigned int rows, unsigned int per, unsigned int piece_rows)
 {
+    __shared__ __align__(16) float4 acc_s[PC_WARPS][K][32];
+    __shared__ float max_s[PC_WARPS][32], sum_s[PC_WARPS][32];
+    const unsigned int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, VL = paged_ld(p.c.vdim), quads = (rows + 3) / 4;
+    const size_t size = paged_piece(piece_rows, p.c.vdim), step = 2 * per * size;
     grid_dependency_launch();
     grid_dependency_wait();
-    const PagedHeader h = p.header[blockIdx.x];
-    if (h.entry == 0) { return; }
-    const unsigned int lane = threadIdx.x & 31, r = blockIdx.y * 4 + (threadIdx.x >> 5), VL = paged_ld(p.c.vdim);
-    const PagedEntry v = paged_entry(p, h.entry - 1);
-    const unsigned int row = h.rt * ROWS + r;
-    if (row >= v.n * p.G) { return; }
-    const size_t size = paged_piece(ROWS, p.c.vdim);
-    auto piece = [&](unsigned int i) { return p.partial + (2 * (size_t)(blockIdx.x + i) + (i == 0 ? 1 : 0)) * size; };
-    float top = -INFINITY;
-    for (unsigned int i = lane; i < h.pieces; i += 32) { top = fmaxf(top, piece(i)[ROWS * VL + r]); }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) { top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o)); }
-    float sum = 0.f;
-    float4 acc[2] = { make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f) };
-#pragma unroll 4
-    for (unsigned int i = 0; i < h.pieces; i++)
+    for (unsigned int c0 = 0; c0 < quads; c0 += 32)
     {
-        const float* x = piece(i);
-        const float c = top == -INFINITY ? 1.f : exp2f(x[ROWS * VL + r] - top);
-        sum = fmaf(c, x[ROWS * VL + ROWS + r], sum);
-#pragma unroll
-        for (unsigned int k = 0; k < 2; k++)
+        // lane i looks at rows 4 (c0 + i) .. of a CTA's segment; every warp does
+        const unsigned int c = c0 + lane, cta = (blockIdx.x + gridDim.x - c % gridDim.x) % gridDim.x;
+        PagedHeader h = {};
+        if (c < quads) { h = p.header[cta]; }
+        unsigned int mask = __ballot_sync(0xFFFFFFFFu, h.pieces != 0 && 4 * c < h.rows);
+        unsigned int team = PC_WARPS;    // warps of a task
+        while (team > 1 && __popc(mask) * team > PC_WARPS) { team >>= 1; }
+        const unsigned int part = warp % team;
+        while (mask != 0)
         {
-            const unsigned int d = lane * 4 + k * 128;
-            if (d < VL)
-            {
-                const float4 y = load4(x + (size_t)r * VL + d);
-                acc[k].x = fmaf(c, y.x, acc[k].x);
-                acc[k].y = fmaf(c, y.y, acc[k].y);
-                acc[k].z = fmaf(c, y.z, acc[k].z);
-                acc[k].w = fmaf(c, y.w, acc[k].w);
-            }
-        }
-    }
-    const unsigned int head = h.kvh * p.G + row % p.G;
-    const float f = paged_factor(p, head, top, sum);
-    T* out = (T*)p.out + (size_t)(v.start + row / p.G) * p.ldo + (size_t)head * p.c.vdim;
-    const bool vec = paged_vec4<T>(p);
+            // the next PC_WARPS / team tasks; this warp's is the (warp / team)-th
+            unsigned int mine = mask;
+            for (unsigned int i = 0; i < warp / team; i++) { mine &= mine - 1; }
+            for (unsigned int i = 0; i < PC_WARPS / team; i++) { mask &= mask - 1; }
+            const bool real = mine != 0;
+            const int from = real ? __ffs(mine) - 1 : 0;
+            const unsigned int pieces = __shfl_sync(0xFFFFFFFFu, h.pieces, from), worker = __shfl_sync(0xFFFFFFFFu, h.worker, from);
+            const unsigned int r = 4 * (c0 + from), all = __shfl_sync(0xFFFFFFFFu, h.rows, from);
+            const float *own = p.partial + (2 * (size_t)worker + 1) * size, *next = p.partial + (size_t)(worker / per + 1) * step;
+            PagedQuad<K> x;
+            x.top = -INFINITY;
+            x.sum = 0.f;
 #pragma unroll
-    for (unsigned int k = 0; k < 2; k++)
-    {
-        const unsigned int d = lane * 4 + k * 128;
-        if (d < p.c.vdim) { paged_store4(out, d, p.c.vdim, vec, make_float4(acc[k].x * f, acc[k].y * f, acc[k].z * f, acc[k].w * f)); }
+            for (int k = 0; k < K; k++) { x.acc[k] = make_float4(0.f, 0.f, 0.f, 0.f); }
+            auto add = [&](float top1, float sum1, const float4* acc1, int stride) {
+                const float top = fmaxf(x.top, top1), f = top == -INFINITY ? 1.f : exp2f(x.top - top), g = top == -INFINITY ? 1.f : exp2f(top1 - top);
+                x.top = top;
+                x.sum = fmaf(x.sum, f, sum1 * g);
+#pragma unroll
+                for (int k = 0; k < K; k++)
+                {
+                    const float4 y = acc1[k * stride];
+                    x.acc[k] = make_float4(fmaf(x.acc[k].x, f, y.x * g), fmaf(x.acc[k].y, f, y.y * g), fmaf(x.acc[k].z, f, y.z * g), fmaf(x.acc[k].w, f, y.w * g));
+                }
+            };
+            // a team's warp takes neighbouring pieces, eight at a time
+            const unsigned int share = (pieces + team - 1) / team, end = real ? min((part + 1) * share, pieces) : 0u;
+            for (unsigned int i = part * share; i < end; i += 8)
+            {
+                const PagedQuad<K> y = paged_join<K>(i == 0 ? own : next + (size_t)(i - 1) * step, next + (size_t)i * step, step, min(8u, end - i), r, all, VL, piece_rows);
+                if (i == part * share) { x = y; }
+                else { add(y.top, y.sum, y.acc, 1); }
+            }
+            if (team > 1)
+            {
+                max_s[warp][lane] = x.top;
+                sum_s[warp][lane] = x.sum;
+#pragma unroll
+                for (int k = 0; k < K; k++) { acc_s[warp][k][lane] = x.acc[k]; }
+                __syncthreads();
+                for (unsigned int i = 1; part == 0 && i < team; i++) { add(max_s[warp + i][lane], sum_s[warp + i][lane], &acc_s[warp + i][0][lane], 32); }
+                __syncthreads();
+            }
+            const unsigned int row = r + (lane >> 3), r0 = __shfl_sync(0xFFFFFFFFu, h.r0, from), kvh = __shfl_sync(0xFFFFFFFFu, h.kvh, from);
+            const unsigned int start = __shfl_sync(0xFFFFFFFFu, h.start, from);
+            paged_put<T>(p, x, start, kvh, r0 + row, real && part == 0 && row < all);
+        }
     }
 }
 
-template <class T, unsigned int ROWS>
-static int combine(const PagedParams& p, unsigned int rows, unsigned int ctas, cudaStream_t stream)
+// rows: the most that a segment has
+template <class T>
+static int combine(const PagedParams& p, unsigned int rows, unsigned int ctas, unsigned int per, unsigned int piece_rows, cudaStream_t stream)
 {
-    return launch_kernel("paged_combine", paged_combine_kernel<T, ROWS>, dim3(ctas, (rows + 3) / 4), dim3(128), 0, stream, true, p);
+    const unsigned int most = rows < piece_rows ? rows : piece_rows;
+    const dim3 grid(ctas), block(PC_THREADS);
+    if (p.c.vdim <= 64) { return launch_kernel("paged_combine", paged_combine_kernel<T, 2>, grid, block, 0, stream, true, p, most, per, piece_rows); }
+    if (p.c.vdim <= 128) { return launch_kernel("paged_combine", paged_combine_kernel<T, 4>, grid, block, 0, stream, true, p, most, per, piece_rows); }
+    return launch_kernel("paged_combine", paged_combine_kernel<T, 8>, grid, block, 0, stream, true, p, most, per, piece_rows);
 }
 
 // ---- dispatch ----------------------------------------------------------------------------------------------------
 // Scratch: a header for each CTA of the kernel that has most of them, then the pieces.
-static size_t header_bytes(unsigned int sms) { return (size_t)sms * kPagedPlainCtas * sizeof(PagedHeader); }
-static size_t work_of(unsigned int sms, unsigned int ctas_per_sm, unsigned int rows, unsigned int vdim)
+static_assert(sizeof(PagedHeader) <= 32, "");
+static size_t header_bytes(unsigned int sms) { return (size_t)sms * kPagedPlainCtas * 32; }
+static size_t work_of(unsigned int sms, unsigned int workers_per_sm, unsigned int rows, unsigned int vdim)
 {
-    return header_bytes(sms) + 2 * (size_t)sms * ctas_per_sm * paged_piece(rows, vdim) * 4;
+    return header_bytes(sms) + 2 * (size_t)sms * workers_per_sm * paged_piece(rows, vdim) * 4;
+}
+// The scratch of the kernel that calls of up to `rows` packed query rows per entry and kv head may take.
+static size_t work_for(unsigned int sms, unsigned int rows, unsigned int vdim)
+{
+    static_assert(kPagedPlainCtas * kPagedPlainRows <= kPagedRowsWarps * 8 && kPagedPlainCtas <= kPagedRowsWarps, "the plain kernel needs less");
+    return work_of(sms, kPagedRowsWarps, rows <= 8 ? 8 : 16, vdim);
 }
 
 template <class T, class C>
@@ -260,7 +298,7 @@ static int run_plain(PagedParams& p, unsigned int rows, unsigned int ctas, cudaS
 {
     p.least = 2 * PP_WARPS;
     const int rc = launch_kernel("paged_plain", paged_plain_kernel<T, C>, dim3(ctas), dim3(PP_THREADS), 0, stream, pdl, p);
-    return rc ? rc : combine<T, PP_ROWS>(p, rows < PP_ROWS ? rows : PP_ROWS, ctas, stream);
+    return rc ? rc : combine<T>(p, rows, ctas, 1, PP_ROWS, stream);
 }
 
 }    // namespace b200
@@ -271,9 +309,7 @@ C_EXPORT unsigned long long cuda_b200_paged_attention_work_bytes(unsigned int H,
 {
     const DecoderDevice* dev = decoder_device();
     if (!dev || Hkv == 0 || H == 0 || (H % Hkv) || vdim == 0 || vdim > 256 || (unsigned long long)max_n * (H / Hkv) > 0x7FFFFFFFull) { return 0; }
-    // the plain kernel and the one for few rows take the same
-    static_assert(kPagedPlainCtas * kPagedPlainRows == kPagedRowsRows, "");
-    return work_of(dev->sm_count, 1, kPagedRowsRows, vdim);
+    return work_for(dev->sm_count, max_n * (H / Hkv), vdim);
 }
 
 C_EXPORT int cuda_b200_paged_attention_rows(int dtype, const cuda_b200_paged_attention* a, const cuda_b200_pages* c, const cuda_b200_batch* b, void* stream,
@@ -305,14 +341,15 @@ C_EXPORT int cuda_b200_paged_attention_rows(int dtype, const cuda_b200_paged_att
     const bool pdl = (flags & 1u) != 0, coded = c->type == DT_E4M3;
     const cudaStream_t st = (cudaStream_t)stream;
     const unsigned int rows = b->max_n * p.G, sms = (unsigned int)dev->sm_count;
-    if (a->work_bytes < work_of(sms, 1, kPagedRowsRows, c->vdim)) { return -1; }
+    if (a->work_bytes < work_for(sms, rows, c->vdim)) { return -1; }
     if (dtype == DT_FLOAT) { kernel = 1; }
     if (kernel == 0) { kernel = 2; }
     if (kernel == 2)
     {
-        const int rc = launch_paged_rows(p, coded, rows, sms, st, pdl);
+        unsigned int per = 0;
+        const int rc = launch_paged_rows(p, coded, rows, sms, &per, st, pdl);
         if (rc) { return rc; }
-        return rows <= 8 ? combine<__nv_bfloat16, 8>(p, rows, sms, st) : combine<__nv_bfloat16, kPagedRowsRows>(p, rows < kPagedRowsRows ? rows : kPagedRowsRows, sms, st);
+        return combine<__nv_bfloat16>(p, rows, sms, per, rows <= 8 ? 8 : 16, st);
     }
     const unsigned int ctas = sms * kPagedPlainCtas;
     if (dtype == DT_FLOAT) { return coded ? run_plain<float, unsigned char>(p, rows, ctas, st, pdl) : run_plain<float, float>(p, rows, ctas, st, pdl); }

@@ -25,10 +25,10 @@ inline bool make_paged_map(CUtensorMap* map, bool coded, const void* base, unsig
         == CUDA_SUCCESS;
 }
 
-// The kernels' segments: packed query rows, CTAs per SM.
-constexpr unsigned int kPagedPlainRows = 4, kPagedPlainCtas = 4, kPagedRowsRows = 16;    // (8 where no entry has more)
+// The plain kernel: packed query rows of a segment, CTAs per SM.  The one for few rows (8 or 16 of them): warps of an SM that take shares.
+constexpr unsigned int kPagedPlainRows = 4, kPagedPlainCtas = 4, kPagedRowsWarps = 8;
 
-// paged_rows.cu: `ctas` CTAs at most, one per SM
-int launch_paged_rows(PagedParams& p, bool coded, unsigned int rows, unsigned int ctas, cudaStream_t stream, bool pdl);
+// paged_rows.cu: a CTA on each of `sms` SMs; *per: its workers
+int launch_paged_rows(PagedParams& p, bool coded, unsigned int rows, unsigned int sms, unsigned int* per, cudaStream_t stream, bool pdl);
 
 }    // namespace b200

@@ -1,10 +1,10 @@
-// How a ragged batch over a cache in pages is dealt out to CTAs, and which keys its rows see.  Nothing here needs a GPU, so that it can
+// How a ragged batch over a cache in pages is dealt out to workers (CTAs, or their warps), and which keys its rows see.  Nothing here needs a GPU, so that it can
 // be looked at without one.
 //
 // A segment is a kv head of an entry with up to ROWS packed query rows (tokens x heads of the kv head); its keys come in units of
 // UNIT, those of the window and, with a window, those of the first keys.  All segments' units lie one behind the other, entry by
-// entry, and every CTA takes an equal share of them: long and short sequences, one sequence or many come out even, and no
-// length has to be known on the host.  A share's segments that are whole are written out; of the (at most two) others the CTA
+// entry, and every worker takes an equal share of them: long and short sequences, one sequence or many come out even, and no
+// length has to be known on the host.  A share's segments that are whole are written out; of the (at most two) others the worker
 // leaves maximum, sum and weighted values in the scratch, and a second kernel puts the pieces together in their order, so that the
 // same call gives the same bits.
 #pragma once
@@ -31,6 +31,12 @@ B200_PLAN T plan_max(T a, T b)
     return a < b ? b : a;
 }
 
+// a / b; the short division where it will do (a long one takes the GPU a hundred instructions)
+B200_PLAN unsigned long long plan_div(unsigned long long a, unsigned long long b)
+{
+    return ((a | b) >> 32) == 0 ? (unsigned int)a / (unsigned int)b : a / b;
+}
+
 struct PagedCache
 {
     unsigned char *k, *v, *k_scale, *v_scale;
@@ -51,14 +57,16 @@ struct PagedPlan
     PagedCache c;
     PagedBatch b;
     unsigned int G, window, first;    // query heads per kv head
-    unsigned int least;               // units a CTA gets at least, where there are enough
+    unsigned int least;               // units a worker gets at least, where there are enough
 };
 
 // The segment that a CTA leaves unfinished.
 struct PagedHeader
 {
-    unsigned int entry, kvh, rt;    // entry + 1; 0: there is none
-    unsigned int pieces;            // its own and the first ones of the CTAs behind it
+    unsigned int pieces;            // its own and those of the CTAs behind it; 0: there is no such segment
+    unsigned int worker;            // that has begun it
+    unsigned int rows, r0;          // packed query rows, the first one
+    unsigned int start, kvh;        // the entry's first token
 };
 
 // The page of a sequence's position, or -1.
@@ -136,20 +144,20 @@ B200_PLAN bool paged_seen(const PagedPlan& p, const PagedEntry& v, unsigned int 
     return key >= v.floor && key <= t && key < p.c.cap && (p.window == 0 || t - key < p.window || key - v.floor < p.first);
 }
 
-// A CTA's share.
+// A worker's share.
 struct PagedShare
 {
     unsigned long long total, begin, end;
-    unsigned int ctas;               // that have a share
+    unsigned int workers;            // that have a share
     unsigned int e, kvh, rt, unit;   // where `begin` lies
 };
-// CTAs that get a share, and where the share of CTA c begins.
-B200_PLAN unsigned int paged_ctas(unsigned long long total, unsigned int least, unsigned int grid)
+// Workers that get a share, and where the share of worker w begins.
+B200_PLAN unsigned int paged_workers(unsigned long long total, unsigned int least, unsigned int most)
 {
-    const unsigned long long fit = total / least;
-    return fit == 0 ? 1u : fit < grid ? (unsigned int)fit : grid;
+    const unsigned long long fit = plan_div(total, least);
+    return fit == 0 ? 1u : fit < most ? (unsigned int)fit : most;
 }
-B200_PLAN unsigned long long paged_begin(unsigned long long total, unsigned int c, unsigned int ctas) { return c < ctas ? total * c / ctas : total; }
+B200_PLAN unsigned long long paged_begin(unsigned long long total, unsigned int w, unsigned int workers) { return w < workers ? plan_div(total * w, workers) : total; }
 
 // Units of one head of an entry.
 template <unsigned int UNIT, unsigned int ROWS>
@@ -174,8 +182,8 @@ B200_PLAN void paged_find(const PagedPlan& p, unsigned int e, unsigned int e_end
             continue;
         }
         share->e = e;
-        share->kvh = (unsigned int)(at / head);
-        at %= head;
+        share->kvh = (unsigned int)plan_div(at, head);
+        at -= share->kvh * head;
         unsigned int rt = 0;
         for (unsigned int n = paged_segment<UNIT, ROWS>(p, v, 0).count; at >= n; n = paged_segment<UNIT, ROWS>(p, v, ++rt).count) { at -= n; }
         share->rt = rt;
@@ -222,11 +230,10 @@ struct PagedCursor
     // Units of the segment in a share of which `left` units are left, and whether that is all of them.
     B200_PLAN unsigned int take(unsigned long long left) const { return (unsigned int)plan_min((unsigned long long)(s.count - unit), left); }
     B200_PLAN bool whole(unsigned int taken) const { return taken == s.count; }
-    // The segment, begun at the global unit `begin` of this CTA, and the pieces it comes in.
-    B200_PLAN PagedHeader header(const PagedShare& share, unsigned long long begin, unsigned int cta) const
+    // The worker whose share holds the segment's last unit, where `begin` is the global unit of the first one in the share.
+    B200_PLAN unsigned int last(const PagedShare& share, unsigned long long begin) const
     {
-        const unsigned long long last = ((begin + s.count) * share.ctas - 1) / share.total;    // the CTA whose share holds its last unit
-        return PagedHeader{ e + 1, kvh, rt, (unsigned int)(last - cta) + 1 };
+        return (unsigned int)plan_div((begin + (s.count - unit)) * share.workers - 1, share.total);
     }
 };
 

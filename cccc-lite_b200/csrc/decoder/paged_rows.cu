@@ -1,7 +1,7 @@
 // Attention of few query rows (up to 16 packed ones per segment: decoding) over a cache in pages, HBM-bound, on mma.sync.
 //
-// Every warp streams units of its own through a ring in shared memory that only it uses: its first lane asks for the pages' rows by
-// TMA, sixteen at a time, and no barrier stands between the warps while they stream.  Both products are turned, so that the few
+// Every warp has a share of the units of its own, a ring in shared memory that only it uses and another warp that asks for the pages' rows by
+// TMA, sixteen at a time: warps never meet, whatever the lengths of the segments.  Both products are turned, so that the few
 // queries are the short side of m16n8k16: sixteen keys, then sixteen elements of values, are the rows.  Scores: a lane takes 16 bytes of
 // two keys' rows as the k places of several products (the queries' elements are permuted alike).  Values: a lane takes the same
 // 16 bytes of four keys; byte permutes pair two keys' elements, two elements make a product's rows.  The weights change their place
@@ -27,7 +27,7 @@ struct RowsShape
 {
     static constexpr int EB = CODED ? 1 : 2;
     static constexpr int ROW = D * EB;                                  // bytes of a cache row
-    static constexpr int WARPS = ROW > 256 ? 4 : 8;
+    static constexpr int WARPS = ROW > 256 ? 4 : (int)kPagedRowsWarps;    // that have a share, and as many that ask
     static constexpr int STAGES = 3;
     static constexpr int UNIT = ROW >= 256 ? 16 : 4096 / ROW;           // keys: 8 KB a stage (16 KB for the longest rows)
     static constexpr int SUB = UNIT / 16;
@@ -42,11 +42,12 @@ struct RowsShape
     static constexpr int STAGE = 2 * UNIT * ROW;
     static constexpr int SCALES = CODED ? 2 * UNIT : 0;                 // exponent bytes of a stage
     static constexpr int INFO = 16;                                     // of a stage: first key, subtiles on no page
-    static constexpr int MERGE = D > 128 ? 2 : 4;                       // rows that the warps put together at a time
-    static constexpr int MERGE_LD = D + 4;
+    // Registers: 96 of a thread at launch, then 144 where shares are worked on and 48 where they are asked for, so that the kernel behind this one
+    // finds room to wait beside it; where that would spill 128, then 200 and 56; with four warps of each kind what there is.
+    __host__ __device__ static constexpr bool lean(int nt) { return WARPS == 8 && nt == 1 && D <= 128; }
     static constexpr int RING = STAGES * STAGE;
     static constexpr int SMALL = STAGES * (SCALES + INFO);
-    static constexpr int SMEM = WARPS * (RING + SMALL) + WARPS * MERGE * MERGE_LD * 4 + 1024;
+    static constexpr int SMEM = WARPS * (RING + SMALL) + 1024;
 };
 
 __device__ __forceinline__ uint2 lds64(uint32_t addr)
@@ -100,105 +101,120 @@ __device__ __forceinline__ uint32_t transposed(uint32_t a)
 
 // NT: tiles of eight query rows
 template <int D, bool CODED, int NT>
-__global__ void __launch_bounds__(32 * RowsShape<D, CODED>::WARPS, 1) paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+__global__ void __launch_bounds__(RowsShape<D, CODED>::lean(NT) ? 640 : 64 * RowsShape<D, CODED>::WARPS, 1) paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
     const __grid_constant__ PagedParams p, unsigned int* status)
 {
     using S = RowsShape<D, CODED>;
-    constexpr unsigned int UNIT = S::UNIT, MERGE = S::MERGE, WARPS = S::WARPS, THREADS = 32 * WARPS, ROWS = 8 * NT;
+    constexpr unsigned int UNIT = S::UNIT, WARPS = S::WARPS, ROWS = 8 * NT;
     constexpr int STEPS = D / 16;
     extern __shared__ unsigned char rw_raw[];
     unsigned char* rw_smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(rw_raw) + 1023) & ~(uintptr_t)1023);
-    __shared__ uint64_t full[WARPS][S::STAGES];
-    __shared__ PagedShare share;
-    __shared__ unsigned long long sums[WARPS];
-    __shared__ PagedCursor<UNIT, ROWS> cur_s;
-    __shared__ float max_s[WARPS][ROWS], sum_s[WARPS][ROWS];
-    const unsigned int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    __shared__ uint64_t full[WARPS][S::STAGES], empty[WARPS][S::STAGES];
+    __shared__ PagedSums<64 * WARPS> sums;
+    __shared__ volatile unsigned int abort_flag;
+    const unsigned int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) % WARPS;
+    const bool asks = threadIdx.x >= 32 * WARPS;
     unsigned char* ring = rw_smem + warp * S::RING;
     unsigned char* small = rw_smem + WARPS * S::RING + warp * S::SMALL;    // per stage: info, exponents of keys, of values
-    float* merge = reinterpret_cast<float*>(rw_smem + WARPS * (S::RING + S::SMALL));
 
     if (threadIdx.x == 0)
     {
-        for (unsigned int i = 0; i < WARPS * S::STAGES; i++) { mbar_init(&full[0][0] + i, 1); }
+        for (unsigned int i = 0; i < WARPS * S::STAGES; i++)
+        {
+            mbar_init(&full[0][0] + i, 1);
+            mbar_init(&empty[0][0] + i, 1);
+        }
+        abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     grid_dependency_launch();
     grid_dependency_wait();
-    paged_share<UNIT, ROWS, THREADS>(p, sums, &share);
-    if (share.begin >= share.end)
+    paged_sums<UNIT, ROWS, 64 * WARPS>(p, &sums);
+    const unsigned int worker = blockIdx.x * WARPS + warp;
+    const PagedShare share = paged_share<UNIT, ROWS, 64 * WARPS>(p, sums, worker, gridDim.x * WARPS);
+    const unsigned int length = (unsigned int)(share.end - share.begin);    // places are counted from the share's first unit on
+    auto wait = [&](uint64_t* bar, unsigned int parity) { return abort_flag == 0 && mbar_wait_bounded(bar, parity & 1u); };
+
+    if (asks)
     {
-        if (threadIdx.x == 0) { p.header[blockIdx.x] = PagedHeader{}; }
+        if constexpr (S::lean(NT)) { asm volatile("setmaxnreg.dec.sync.aligned.u32 48;"); }
+        else if constexpr (WARPS == 8) { asm volatile("setmaxnreg.dec.sync.aligned.u32 56;"); }
+        if (lane != 0 || length == 0) { return; }
+        PagedCursor<UNIT, ROWS> cur;
+        cur.at(p, share);
+        unsigned int seg = 0, key = 0;    // where the segment's units in the share begin; the unit's first key
+        int page[S::SUB];                 // of its sixteens, as the table has them: they are looked at when the unit before has been asked for
+        auto find = [&](unsigned int at) {
+            for (unsigned int n = cur.s.count - cur.unit; at - seg >= n; n = cur.s.count)
+            {
+                seg += n;
+                cur.next(p);
+            }
+            key = cur.s.unit(cur.unit + (at - seg)) * UNIT;
+#pragma unroll
+            for (int i = 0; i < S::SUB; i++)
+            {
+                const unsigned int first = key + i * 16;
+                page[i] = -1;
+                // sixteen keys meet one of the two wanted ranges (there is none for a slot that is none, or behind the table's row)
+                if (first < cur.s.lim && (first + 16 > cur.s.low || (first + 16 > cur.v.floor && first < cur.s.first_end)))
+                {
+                    page[i] = p.c.table[(size_t)(unsigned int)cur.v.slot * p.c.ld_table + (first >> p.c.shift)];
+                }
+            }
+        };
+        find(0);
+        unsigned int at = 0;
+        bool ok = true;
+        for (; at < length; at++)
+        {
+            const unsigned int stage = at % S::STAGES;
+            if (at >= (unsigned int)S::STAGES && !wait(&empty[warp][stage], at / S::STAGES - 1))
+            {
+                ok = false;
+                break;
+            }
+            uint64_t* bar = &full[warp][stage];
+            unsigned char *to = ring + stage * S::STAGE, *info = small + stage * (S::INFO + S::SCALES);
+            unsigned int bad = 0;
+#pragma unroll
+            for (int i = 0; i < S::SUB; i++) { bad |= ((unsigned int)page[i] >= p.c.pages ? 1u : 0u) << i; }
+            *reinterpret_cast<uint2*>(info) = make_uint2(key, bad);
+            mbar_expect_tx(bar, S::STAGE + (CODED ? 32 * (S::SUB - __popc(bad)) : 0));
+#pragma unroll
+            for (int i = 0; i < S::SUB; i++)
+            {
+                const unsigned int row = (cur.kvh << p.c.shift) + ((key + i * 16) & ((1u << p.c.shift) - 1u));
+                const bool none = (bad >> i & 1u) != 0;
+                const int z = none ? (int)p.c.pages : page[i];    // behind the caches' end: zeros
+#pragma unroll
+                for (int b = 0; b < S::BOXES; b++)
+                {
+                    tma_load_3d(to + (i * S::BOXES + b) * S::BOX, &tmK, b * (128 / S::EB), (int)row, z, bar);
+                    tma_load_3d(to + UNIT * S::ROW + (i * S::BOXES + b) * S::BOX, &tmV, b * (128 / S::EB), (int)row, z, bar);
+                }
+                if (CODED && !none)
+                {
+                    const size_t from = ((size_t)(unsigned int)z * p.c.Hkv << p.c.shift) + row;
+                    bulk_g2s(info + S::INFO + i * 16, p.c.k_scale + from, 16, bar);
+                    bulk_g2s(info + S::INFO + UNIT + i * 16, p.c.v_scale + from, 16, bar);
+                }
+            }
+            mbar_arrive(bar);
+            if (at + 1 < length) { find(at + 1); }
+        }
+        if (!ok)
+        {
+            note_timeout(status, WAIT_PAGED_ROWS, 8u + (warp & 7u), at);
+            abort_flag = 1;
+        }
+        // whatever the other warp does, the copies in flight arrive (bounded) before the CTA may leave
+        for (unsigned int i = at < (unsigned int)S::STAGES ? 0 : at - S::STAGES; i < at; i++) { mbar_wait_bounded(&full[warp][i % S::STAGES], (i / S::STAGES) & 1u); }
         return;
     }
-    const unsigned int end = (unsigned int)(share.end - share.begin);    // places are counted from the share's first unit on
-
-    // ---- what the warp asks for: units warp, warp + WARPS, ... of the share, across its segments ----
-    PagedCursor<UNIT, ROWS> ask;
-    unsigned int ask_at = warp, ask_seg = 0;    // the unit, and where its segment's units in the share begin
-    ask.at(p, share);
-    unsigned int ask_key = 0;
-    int ask_page = -1;    // lane i: the page of the unit's i-th sixteen keys as the table has it; looked at only when it is needed, a unit later
-    auto find = [&]() {
-        if (ask_at >= end) { return; }
-        for (unsigned int n = ask.s.count - ask.unit; ask_at - ask_seg >= n; n = ask.s.count)
-        {
-            ask_seg += n;
-            ask.next(p);
-        }
-        ask_key = ask.s.unit(ask.unit + (ask_at - ask_seg)) * UNIT;
-        const unsigned int first = ask_key + lane * 16;
-        ask_page = -1;
-        // a range of keys meets one of the two wanted ranges
-        if (lane < (unsigned int)S::SUB && first < ask.s.lim && (first + 16 > ask.s.low || (first + 16 > ask.v.floor && first < ask.s.first_end)))
-        {
-            const unsigned int i = first >> p.c.shift;    // (lim is 0 for a slot that is none, and nowhere behind the table's row)
-            ask_page = p.c.table[(size_t)(unsigned int)ask.v.slot * p.c.ld_table + i];
-        }
-    };
-    unsigned int asked = 0;    // units
-    auto request = [&]() {
-        if (ask_at >= end) { return; }
-        const unsigned int stage = asked % S::STAGES;
-        unsigned char* to = ring + stage * S::STAGE;
-        unsigned char* info = small + stage * (S::INFO + S::SCALES);
-        const bool none = (unsigned int)ask_page >= p.c.pages;
-        const unsigned int bad = __ballot_sync(0xFFFFFFFFu, lane < (unsigned int)S::SUB && none);
-        if (none) { ask_page = (int)p.c.pages; }    // behind the caches' end: zeros
-        if (lane == 0)
-        {
-            *reinterpret_cast<uint2*>(info) = make_uint2(ask_key, bad);
-            mbar_expect_tx(&full[warp][stage], S::STAGE + (CODED ? 32 * (S::SUB - __popc(bad)) : 0));
-        }
-        __syncwarp();
-        // lane i asks for the i-th sixteen keys
-        if (lane < (unsigned int)S::SUB)
-        {
-            const unsigned int at = (ask.kvh << p.c.shift) + ((ask_key + lane * 16) & ((1u << p.c.shift) - 1u));
-#pragma unroll
-            for (int i = 0; i < S::BOXES; i++)
-            {
-                tma_load_3d(to + (lane * S::BOXES + i) * S::BOX, &tmK, i * (128 / S::EB), (int)at, ask_page, &full[warp][stage]);
-                tma_load_3d(to + UNIT * S::ROW + (lane * S::BOXES + i) * S::BOX, &tmV, i * (128 / S::EB), (int)at, ask_page, &full[warp][stage]);
-            }
-            if (CODED && !none)
-            {
-                const size_t from = ((size_t)(unsigned int)ask_page * p.c.Hkv << p.c.shift) + at;
-                bulk_g2s(info + S::INFO + lane * 16, p.c.k_scale + from, 16, &full[warp][stage]);
-                bulk_g2s(info + S::INFO + UNIT + lane * 16, p.c.v_scale + from, 16, &full[warp][stage]);
-            }
-        }
-        __syncwarp();
-        if (lane == 0) { mbar_arrive(&full[warp][stage]); }
-        asked++;
-        ask_at += WARPS;
-        find();
-    };
-    find();
-#pragma unroll
-    for (int s = 0; s + 1 < S::STAGES; s++) { request(); }
-    unsigned int taken = 0;    // units
-    bool lost = false;         // a wait has run out: nothing more is taken
+    if constexpr (S::lean(NT)) { asm volatile("setmaxnreg.inc.sync.aligned.u32 144;"); }
+    else if constexpr (WARPS == 8) { asm volatile("setmaxnreg.inc.sync.aligned.u32 200;"); }
+    const unsigned int g = lane >> 2, t = lane & 3;
     // Rows of the products: key `order(i)` of eight is row i.  Where a lane finds its pieces of a copy.
     auto order = [](unsigned int i) { return (i >> 1) ^ ((i & 1u) * (S::WIDE ? 4u : 5u)); };
     const unsigned int key_g = order(g);
@@ -213,15 +229,22 @@ __global__ void __launch_bounds__(32 * RowsShape<D, CODED>::WARPS, 1) paged_rows
     }
     const uint32_t pair[2] = { CODED ? (swap ? 0x1504u : 0x5140u) : (swap ? 0x1054u : 0x5410u), CODED ? (swap ? 0x3726u : 0x7362u) : (swap ? 0x3276u : 0x7632u) };
 
-    if (threadIdx.x == 0) { cur_s.at(p, share); }
-    PagedHeader header = {};
-    unsigned int at = 0, mine = warp;    // the segment's first unit; the warp's next unit
-    while (at < end)
+    PagedCursor<UNIT, ROWS> cur;
+    if (length != 0) { cur.at(p, share); }
+    const unsigned int size = (unsigned int)paged_piece(ROWS, p.c.vdim), VL = paged_ld(p.c.vdim);
+    float* pieces = p.partial + 2 * (size_t)worker * size;
+    // The CTA's pieces of a segment that a CTA before has begun (this warp's first, where it is the first one), and those of a segment that this
+    // warp has begun and not finished: how many workers' of this CTA.
+    unsigned int inherited = 0, begun = 0, begun_last = 0;
+    const unsigned int inherited_rows = length != 0 ? cur.s.rows : 0u;
+    if (warp == 0 && length != 0 && cur.unit != 0) { inherited = min(cur.last(share, share.begin) - worker + 1, WARPS); }
+    unsigned int taken = 0;    // units
+    bool lost = false;         // a wait has run out
+    for (unsigned int at = 0; at < length && !lost;)
     {
-        __syncthreads();
-        const PagedEntry v = cur_s.v;
-        const PagedSegment s = cur_s.s;
-        const unsigned int kvh = cur_s.kvh, units = cur_s.take(end - at);
+        const PagedEntry& v = cur.v;
+        const PagedSegment& s = cur.s;
+        const unsigned int kvh = cur.kvh, units = cur.take(length - at);
         // ---- queries: row g of each tile as an operand; the scores' columns are the rows 2 t and 2 t + 1 ----
         uint32_t q[NT][STEPS][2];
         float rs[NT][2];
@@ -297,16 +320,14 @@ __global__ void __launch_bounds__(32 * RowsShape<D, CODED>::WARPS, 1) paged_rows
         const unsigned int lim_all = min(v.pos + s.r0 / p.G + 1, s.lim), t_last = v.pos + (s.r0 + s.rows - 1) / p.G;
         const unsigned int low_all = max(v.floor, p.window != 0 && t_last + 1 > p.window ? t_last + 1 - p.window : 0u);
 
-        for (; mine < at + units; mine += WARPS)
+        for (; taken < at + units; taken++)
         {
             const unsigned int stage = taken % S::STAGES;
-            if (!__all_sync(0xFFFFFFFFu, !lost && mbar_wait_bounded(&full[warp][stage], (taken / S::STAGES) & 1u)))
+            if (!__all_sync(0xFFFFFFFFu, wait(&full[warp][stage], taken / S::STAGES)))
             {
-                if (!lost && lane == 0) { note_timeout(status, WAIT_PAGED_ROWS, warp & 15u, taken); }
                 lost = true;
                 break;
             }
-            request();    // into the place of the unit before this one, which every lane is done with
             const uint32_t from = smem_u32(ring) + stage * S::STAGE, from_v = from + UNIT * S::ROW;
             const uint32_t info = smem_u32(small) + stage * (S::INFO + S::SCALES);
             const uint2 what = lds64(info);
@@ -535,135 +556,132 @@ __global__ void __launch_bounds__(32 * RowsShape<D, CODED>::WARPS, 1) paged_rows
                     }
                 }
             }
-            taken++;
             __syncwarp();
+            if (lane == 0) { mbar_arrive(&empty[warp][stage]); }
         }
 
-        // ---- the warps' parts together, a few rows at a time ----
+        // ---- the segment's outputs, or its piece: a lane has its pieces' elements of the rows 2 t and 2 t + 1 ----
+        const bool whole = cur.whole(units), vec = paged_vec4<__nv_bfloat16>(p);
+        float* piece = pieces + (cur.unit == 0 ? size : 0u);
 #pragma unroll
         for (int n = 0; n < NT; n++)
         {
 #pragma unroll
             for (int x = 0; x < 2; x++)
             {
+                float sum = l[n][x];
 #pragma unroll
-                for (int o = 4; o < 32; o <<= 1) { l[n][x] += __shfl_xor_sync(0xFFFFFFFFu, l[n][x], o); }
-                if (g == 0)
+                for (int o = 4; o < 32; o <<= 1) { sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o); }
+                const unsigned int r = n * 8 + 2 * t + x, row = s.r0 + r, head = kvh * p.G + row % p.G;
+                if (r >= s.rows) { continue; }
+                const float f = whole ? paged_factor(p, head, m[n][x], sum) : 1.f;
+                __nv_bfloat16* out = (__nv_bfloat16*)p.out + (size_t)(v.start + row / p.G) * p.ldo + (size_t)head * p.c.vdim;
+#pragma unroll
+                for (int i = 0; i < S::VI; i++)
                 {
-                    max_s[warp][n * 8 + 2 * t + x] = m[n][x];
-                    sum_s[warp][n * 8 + 2 * t + x] = l[n][x];
-                }
-            }
-        }
-        const bool whole = cur_s.whole(units);
-        const unsigned int VL = paged_ld(p.c.vdim);
-        float* piece = p.partial + (2 * (size_t)blockIdx.x + (cur_s.unit == 0 ? 1 : 0)) * paged_piece(ROWS, p.c.vdim);
-        const bool vec = paged_vec4<__nv_bfloat16>(p);
-        for (unsigned int r0 = 0; r0 < s.rows; r0 += MERGE)
-        {
-            if (r0 != 0) { __syncthreads(); }
 #pragma unroll
-            for (int n = 0; n < NT; n++)
-            {
-#pragma unroll
-                for (int y = 0; y < 2; y++)
-                {
-                    const unsigned int r = n * 8 + 2 * t + y - r0;
-                    if (r < MERGE)
+                    for (int j = 0; j < S::VE / 2; j += 2)
                     {
-                        float* to = merge + (warp * MERGE + r) * S::MERGE_LD;
-#pragma unroll
-                        for (int i = 0; i < S::VI; i++)
+                        const int k = i * S::VE / 2 + j;
+                        const unsigned int d = (i * 8 + g) * S::VE + 2 * j;
+                        const float4 o = make_float4(acc[k][n][x] * f, acc[k][n][2 + x] * f, acc[k + 1][n][x] * f, acc[k + 1][n][2 + x] * f);
+                        if (!whole)
                         {
-#pragma unroll
-                            for (int x = 0; x < S::VE / 2; x += 2)
-                            {
-                                const int k = i * S::VE / 2 + x;
-                                store4(to + (i * 8 + g) * S::VE + 2 * x, make_float4(acc[k][n][y], acc[k][n][2 + y], acc[k + 1][n][y], acc[k + 1][n][2 + y]));
-                            }
+                            if (d < VL) { store4(piece + (size_t)r * VL + d, o); }
                         }
+                        else if (d < p.c.vdim) { paged_store4(out, d, p.c.vdim, vec, o); }
                     }
                 }
-            }
-            __syncthreads();
-            const unsigned int rows = min(MERGE, s.rows - r0);
-            for (unsigned int i = threadIdx.x; i < rows * (VL / 4); i += THREADS)
-            {
-                const unsigned int r = i / (VL / 4), d = i % (VL / 4) * 4;
-                float most = -INFINITY, sum = 0.f;
-#pragma unroll
-                for (unsigned int x = 0; x < WARPS; x++) { most = fmaxf(most, max_s[x][r0 + r]); }
-                float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-                for (unsigned int x = 0; x < WARPS; x++)
+                if (!whole && g == 0)
                 {
-                    const float f = most == -INFINITY ? 1.f : paged_exp2(max_s[x][r0 + r] - most);
-                    const float4 y = load4(merge + (x * MERGE + r) * S::MERGE_LD + d);
-                    sum = fmaf(f, sum_s[x][r0 + r], sum);
-                    o.x = fmaf(f, y.x, o.x);
-                    o.y = fmaf(f, y.y, o.y);
-                    o.z = fmaf(f, y.z, o.z);
-                    o.w = fmaf(f, y.w, o.w);
-                }
-                if (whole)
-                {
-                    const unsigned int row = s.r0 + r0 + r, head = kvh * p.G + row % p.G;
-                    const float f = paged_factor(p, head, most, sum);
-                    if (d < p.c.vdim)
-                    {
-                        paged_store4((__nv_bfloat16*)p.out + (size_t)(v.start + row / p.G) * p.ldo + (size_t)head * p.c.vdim, d, p.c.vdim, vec,
-                            make_float4(o.x * f, o.y * f, o.z * f, o.w * f));
-                    }
-                }
-                else
-                {
-                    store4(piece + (size_t)(r0 + r) * VL + d, o);
-                    if (d == 0)
-                    {
-                        piece[ROWS * VL + r0 + r] = most;
-                        piece[ROWS * VL + ROWS + r0 + r] = sum;
-                    }
+                    piece[ROWS * VL + r] = m[n][x];
+                    piece[ROWS * VL + ROWS + r] = sum;
                 }
             }
         }
-        if (!whole && cur_s.unit == 0) { header = cur_s.header(share, share.begin + at, blockIdx.x); }
+        if (!whole && cur.unit == 0)
+        {
+            begun_last = cur.last(share, share.begin + at);
+            begun = min(begun_last - worker + 1, WARPS - warp);
+        }
         at += units;
-        __syncthreads();
-        if (threadIdx.x == 0 && at < end) { cur_s.next(p); }
+        if (at < length) { cur.next(p); }
     }
     if (lost && lane == 0)
     {
-        // wait (bounded) for the copies in flight before the CTA may leave
-        for (; taken < asked; taken++) { mbar_wait_bounded(&full[warp][taken % S::STAGES], (taken / S::STAGES) & 1u); }
+        note_timeout(status, WAIT_PAGED_ROWS, warp & 7u, taken);
+        abort_flag = 1;
     }
-    if (threadIdx.x == 0) { p.header[blockIdx.x] = header; }
+
+    // ---- the CTA's pieces of a segment together: an output, or one piece of the CTA (the header's segment is begun here and goes on behind it) ----
+    if (threadIdx.x == 0) { p.header[blockIdx.x] = PagedHeader{}; }
+    asm volatile("bar.sync 1, %0;" ::"n"(32 * WARPS) : "memory");
+    const float* behind = pieces + 2 * size;    // the next warp's first piece
+    constexpr int K = D / 32;
+    auto leave = [&](float* piece, const PagedQuad<K>& x, unsigned int r, unsigned int rows) {
+        const unsigned int row = r + (lane >> 3), e = lane & 7u;
+        if (row >= rows) { return; }
+#pragma unroll
+        for (unsigned int k = 0; k < (unsigned int)K; k++)
+        {
+            if (k * 32 + e * 4 < VL) { store4(piece + row * VL + k * 32 + e * 4, x.acc[k]); }
+        }
+        if (e == 0)
+        {
+            piece[ROWS * VL + row] = x.top;
+            piece[ROWS * VL + ROWS + row] = x.sum;
+        }
+    };
+    if (inherited > 1)
+    {
+        for (unsigned int r = 0; r < inherited_rows; r += 4)
+        {
+            const PagedQuad<K> x = paged_join<K>(pieces, behind, 2 * size, inherited, r, inherited_rows, VL, ROWS);
+            leave(pieces, x, r, inherited_rows);
+        }
+    }
+    if (begun != 0)    // the cursor is at that segment still
+    {
+        const unsigned int rows = cur.s.rows;
+        const bool done = worker + begun > begun_last;
+        if (!done && lane == 0)
+        {
+            p.header[blockIdx.x] = PagedHeader{ 1 + (begun_last - worker - begun) / WARPS + 1, worker, rows, cur.s.r0, cur.v.start, cur.kvh };
+        }
+        for (unsigned int r = 0; r < rows && (done || begun > 1); r += 4)
+        {
+            const PagedQuad<K> x = paged_join<K>(pieces + size, behind, 2 * size, begun, r, rows, VL, ROWS);
+            if (done) { paged_put<__nv_bfloat16>(p, x, cur.v.start, cur.kvh, cur.s.r0 + r + (lane >> 3), r + (lane >> 3) < rows); }
+            else { leave(pieces + size, x, r, rows); }
+        }
+    }
 }
 
 template <int D, bool CODED>
-static int run_rows(PagedParams& p, unsigned int rows, unsigned int ctas, cudaStream_t stream, bool pdl)
+static int run_rows(PagedParams& p, unsigned int rows, unsigned int sms, unsigned int* per, cudaStream_t stream, bool pdl)
 {
     using S = RowsShape<D, CODED>;
-    p.least = S::WARPS;    // a unit for every warp
-    const dim3 grid(ctas), block(32 * S::WARPS);
+    p.least = 1;
+    *per = S::WARPS;
     unsigned int* status = decoder_status_word();
     if (!status) { return 1; }
     CUtensorMap tk, tv;
     const unsigned int cols = (S::WIDE ? 128 : 64) / S::EB;
     if (!make_paged_map(&tk, CODED, p.c.k, p.c.k_ld, p.c, cols, 16, S::WIDE) || !make_paged_map(&tv, CODED, p.c.v, p.c.v_ld, p.c, cols, 16, S::WIDE)) { return -1; }
+    const dim3 grid(sms), block(64 * S::WARPS);
     return rows <= 8 ? launch_kernel("paged_rows", paged_rows_kernel<D, CODED, 1>, grid, block, (size_t)S::SMEM, stream, pdl, tk, tv, p, status)
                      : launch_kernel("paged_rows", paged_rows_kernel<D, CODED, 2>, grid, block, (size_t)S::SMEM, stream, pdl, tk, tv, p, status);
 }
 
-int launch_paged_rows(PagedParams& p, bool coded, unsigned int rows, unsigned int ctas, cudaStream_t stream, bool pdl)
+int launch_paged_rows(PagedParams& p, bool coded, unsigned int rows, unsigned int sms, unsigned int* per, cudaStream_t stream, bool pdl)
 {
     const unsigned int width = p.c.dim > p.c.vdim ? p.c.dim : p.c.vdim;
-    if (coded)
-    {
-        return width <= 64 ? run_rows<64, true>(p, rows, ctas, stream, pdl) : width <= 128 ? run_rows<128, true>(p, rows, ctas, stream, pdl)
-                                                                                           : run_rows<256, true>(p, rows, ctas, stream, pdl);
-    }
-    return width <= 64 ? run_rows<64, false>(p, rows, ctas, stream, pdl) : width <= 128 ? run_rows<128, false>(p, rows, ctas, stream, pdl)
-                                                                                        : run_rows<256, false>(p, rows, ctas, stream, pdl);
+    auto by_width = [&](auto c) {
+        constexpr bool CODED = decltype(c)::value;
+        return width <= 64 ? run_rows<64, CODED>(p, rows, sms, per, stream, pdl) : width <= 128 ? run_rows<128, CODED>(p, rows, sms, per, stream, pdl)
+                                                                                                   : run_rows<256, CODED>(p, rows, sms, per, stream, pdl);
+    };
+    return coded ? by_width(std::true_type()) : by_width(std::false_type());
 }
 
 }    // namespace b200

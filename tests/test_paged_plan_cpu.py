@@ -1,4 +1,4 @@
-"""How a ragged batch over a paged cache is dealt out to CTAs, and what the calls refuse.  No GPU needed: the rules are host code, and
+"""How a ragged batch over a paged cache is dealt out to workers, and what the calls refuse.  No GPU needed: the rules are host code, and
 a refused call launches nothing."""
 import ctypes as C
 import subprocess
@@ -17,7 +17,7 @@ def plan(tmp_path_factory):
     (top / "plan.cpp").write_text('''
 #include "%s/cccc-lite_b200/csrc/decoder/paged_plan.cuh"
 using namespace b200;
-// Walks every CTA's share.  hits[e][kvh][token][key]: times a row that sees the key meets it (the first head of the token); taken[e][kvh][key]:
+// Walks every worker's share.  hits[e][kvh][token][key]: times a row that sees the key meets it (the first head of the token); taken[e][kvh][key]:
 // the key's row is fetched.  Returns the number of rules that were broken.
 template <unsigned U, unsigned R>
 static int walk(const PagedPlan& p, unsigned grid, unsigned max_t, unsigned max_k, int* hits, int* fetched, int* pieces)
@@ -25,13 +25,13 @@ static int walk(const PagedPlan& p, unsigned grid, unsigned max_t, unsigned max_
     int bad = 0;
     unsigned long long total = 0;
     for (unsigned e = p.b.e0; e < p.b.e0 + p.b.entries; e++) { total += paged_head_units<U, R>(p, paged_entry(p, e)) * p.c.Hkv; }
-    const unsigned ctas = paged_ctas(total, p.least, grid);
+    const unsigned ctas = paged_workers(total, p.least, grid);
     unsigned expect = 0;    // pieces of an unfinished segment still to come
-    PagedHeader open = {};
+    struct { unsigned e, kvh, rt, last; } open = {};
     for (unsigned c = 0; c < grid; c++)
     {
         PagedShare s = {};
-        s.total = total, s.ctas = ctas, s.begin = paged_begin(total, c, ctas), s.end = paged_begin(total, c + 1, ctas);
+        s.total = total, s.workers = ctas, s.begin = paged_begin(total, c, ctas), s.end = paged_begin(total, c + 1, ctas);
         if (c >= ctas && s.begin != s.end) { bad++; }
         if (s.begin >= s.end) { continue; }
         if (s.end - s.begin > (total + ctas - 1) / ctas || (total / p.least >= 1 && s.end - s.begin < p.least)) { bad++; }
@@ -44,18 +44,18 @@ static int walk(const PagedPlan& p, unsigned grid, unsigned max_t, unsigned max_
             const unsigned units = cur.take(s.end - at);
             if (units == 0 || cur.v.n == 0 || cur.e >= p.b.e0 + p.b.entries) { return bad + 1000; }
             const bool whole = cur.whole(units);
-            if (cur.unit != 0)    // a piece of the segment that a CTA before left open
+            if (cur.unit != 0)    // a piece of the segment that a worker before left open
             {
-                if (!first || expect == 0 || open.entry != cur.e + 1 || open.kvh != cur.kvh || open.rt != cur.rt) { bad++; }
+                if (!first || expect == 0 || open.e != cur.e || open.kvh != cur.kvh || open.rt != cur.rt || cur.last(s, at) != open.last) { bad++; }
                 expect--;
                 if ((cur.unit + units == cur.s.count) != (expect == 0)) { bad++; }
             }
             else if (!whole)
             {
                 if (expect != 0) { bad++; }
-                open = cur.header(s, at, c);
-                expect = open.pieces - 1;
-                if (at + units != s.end || open.pieces < 2) { bad++; }
+                open = { cur.e, cur.kvh, cur.rt, cur.last(s, at) };
+                expect = open.last - c;
+                if (at + units != s.end || open.last <= c || open.last >= ctas) { bad++; }
                 pieces[0]++;
             }
             for (unsigned u = 0; u < units; u++)
