@@ -190,8 +190,8 @@ __global__ void __launch_bounds__(PP_THREADS) paged_plain_kernel(const __grid_co
 
 // ---- pieces together ---------------------------------------------------------------------------------------------
 // The segments that CTAs left unfinished: the piece of the worker that has begun it, then the first pieces of the CTAs behind it, in their
-// order.  A task is four rows of such a segment, rows 4 i .. of CTA w's the task of CTA (w + i) % gridDim.x, so that few segments still reach
-// many CTAs.  A task's pieces are dealt to a team of warps (a sequence alone comes in a piece from every CTA), whose parts meet in
+// order.  A task is four rows of such a segment, rows 4 i .. of worker CTA w's the task of CTA (w + i / gridDim.y) % gridDim.x, i % gridDim.y,
+// so that few segments still reach many CTAs.  A task's pieces are dealt to a team of warps (a sequence alone comes in a piece from every CTA), whose parts meet in
 // shared memory, again in order.  Small enough to wait beside the kernel before it on an SM.
 constexpr unsigned int PC_WARPS = 4, PC_THREADS = 32 * PC_WARPS;
 
@@ -201,17 +201,17 @@ __global__ void __launch_bounds__(PC_THREADS, 4) paged_combine_kernel(const __gr
 {
     __shared__ __align__(16) float4 acc_s[PC_WARPS][K][32];
     __shared__ float max_s[PC_WARPS][32], sum_s[PC_WARPS][32];
-    const unsigned int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, VL = paged_ld(p.c.vdim), quads = (rows + 3) / 4;
+    const unsigned int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, VL = paged_ld(p.c.vdim), quads = ((rows + 3) / 4 + gridDim.y - 1) / gridDim.y;    // for a CTA to look at
     const size_t size = paged_piece(piece_rows, p.c.vdim), step = 2 * per * size;
     grid_dependency_launch();
     grid_dependency_wait();
     for (unsigned int c0 = 0; c0 < quads; c0 += 32)
     {
-        // lane i looks at rows 4 (c0 + i) .. of a CTA's segment; every warp does
+        // lane i looks at four rows of a worker CTA's segment; every warp does
         const unsigned int c = c0 + lane, cta = (blockIdx.x + gridDim.x - c % gridDim.x) % gridDim.x;
         PagedHeader h = {};
         if (c < quads) { h = p.header[cta]; }
-        unsigned int mask = __ballot_sync(0xFFFFFFFFu, h.pieces != 0 && 4 * c < h.rows);
+        unsigned int mask = __ballot_sync(0xFFFFFFFFu, h.pieces != 0 && 4 * (c * gridDim.y + blockIdx.y) < h.rows);
         unsigned int team = PC_WARPS;    // warps of a task
         while (team > 1 && __popc(mask) * team > PC_WARPS) { team >>= 1; }
         const unsigned int part = warp % team;
@@ -224,7 +224,7 @@ __global__ void __launch_bounds__(PC_THREADS, 4) paged_combine_kernel(const __gr
             const bool real = mine != 0;
             const int from = real ? __ffs(mine) - 1 : 0;
             const unsigned int pieces = __shfl_sync(0xFFFFFFFFu, h.pieces, from), worker = __shfl_sync(0xFFFFFFFFu, h.worker, from);
-            const unsigned int r = 4 * (c0 + from), all = __shfl_sync(0xFFFFFFFFu, h.rows, from);
+            const unsigned int r = 4 * ((c0 + from) * gridDim.y + blockIdx.y), all = __shfl_sync(0xFFFFFFFFu, h.rows, from);
             const float *own = p.partial + (2 * (size_t)worker + 1) * size, *next = p.partial + (size_t)(worker / per + 1) * step;
             PagedQuad<K> x;
             x.top = -INFINITY;
@@ -272,7 +272,7 @@ template <class T>
 static int combine(const PagedParams& p, unsigned int rows, unsigned int ctas, unsigned int per, unsigned int piece_rows, cudaStream_t stream)
 {
     const unsigned int most = rows < piece_rows ? rows : piece_rows;
-    const dim3 grid(ctas), block(PC_THREADS);
+    const dim3 grid(ctas, most > 16 ? 4 : 1), block(PC_THREADS);    // (a CTA of 128 threads finds room beside the one before it)
     if (p.c.vdim <= 64) { return launch_kernel("paged_combine", paged_combine_kernel<T, 2>, grid, block, 0, stream, true, p, most, per, piece_rows); }
     if (p.c.vdim <= 128) { return launch_kernel("paged_combine", paged_combine_kernel<T, 4>, grid, block, 0, stream, true, p, most, per, piece_rows); }
     return launch_kernel("paged_combine", paged_combine_kernel<T, 8>, grid, block, 0, stream, true, p, most, per, piece_rows);
@@ -290,7 +290,8 @@ static size_t work_of(unsigned int sms, unsigned int workers_per_sm, unsigned in
 static size_t work_for(unsigned int sms, unsigned int rows, unsigned int vdim)
 {
     static_assert(kPagedPlainCtas * kPagedPlainRows <= kPagedRowsWarps * 8 && kPagedPlainCtas <= kPagedRowsWarps, "the plain kernel needs less");
-    return work_of(sms, kPagedRowsWarps, rows <= 8 ? 8 : 16, vdim);
+    const size_t few = work_of(sms, kPagedRowsWarps, rows <= 8 ? 8 : 16, vdim), many = rows <= kPagedFewRows ? 0 : work_of(sms, 1, 256, vdim);
+    return few > many ? few : many;
 }
 
 template <class T, class C>
@@ -320,7 +321,7 @@ C_EXPORT int cuda_b200_paged_attention_rows(int dtype, const cuda_b200_paged_att
     PagedParams p;
     if (!a->q || !a->out || !a->work || !make_paged_cache(dtype, c, &p.c) || !make_paged_batch(b, &p.b)) { return -1; }
     if (a->H == 0 || (a->H % c->Hkv) || a->ldq < (unsigned long long)a->H * c->dim || a->ldo < (unsigned long long)a->H * c->vdim
-        || (unsigned long long)b->max_n * (a->H / c->Hkv) > 0x7FFFFFFFull || (reinterpret_cast<uintptr_t>(a->work) & 15u) || kernel < 0 || kernel > 2)
+        || (unsigned long long)b->max_n * (a->H / c->Hkv) > 0x7FFFFFFFull || (reinterpret_cast<uintptr_t>(a->work) & 15u) || kernel < 0 || kernel > 3)
     {
         return -1;
     }
@@ -343,13 +344,20 @@ C_EXPORT int cuda_b200_paged_attention_rows(int dtype, const cuda_b200_paged_att
     const unsigned int rows = b->max_n * p.G, sms = (unsigned int)dev->sm_count;
     if (a->work_bytes < work_for(sms, rows, c->vdim)) { return -1; }
     if (dtype == DT_FLOAT) { kernel = 1; }
-    if (kernel == 0) { kernel = 2; }
+    if (kernel == 0) { kernel = rows <= kPagedFewRows ? 2 : 3; }
+    if (kernel == 3 && a->work_bytes < work_of(sms, 1, 256, c->vdim)) { return -1; }
     if (kernel == 2)
     {
         unsigned int per = 0;
         const int rc = launch_paged_rows(p, coded, rows, sms, &per, st, pdl);
         if (rc) { return rc; }
         return combine<__nv_bfloat16>(p, rows, sms, per, rows <= 8 ? 8 : 16, st);
+    }
+    if (kernel == 3)
+    {
+        unsigned int piece_rows = 0;
+        const int rc = launch_paged_tile(p, coded, sms, &piece_rows, st, pdl);
+        return rc ? rc : combine<__nv_bfloat16>(p, rows, sms, 1, piece_rows, st);
     }
     const unsigned int ctas = sms * kPagedPlainCtas;
     if (dtype == DT_FLOAT) { return coded ? run_plain<float, unsigned char>(p, rows, ctas, st, pdl) : run_plain<float, float>(p, rows, ctas, st, pdl); }

@@ -27,8 +27,13 @@ inline bool make_paged_map(CUtensorMap* map, bool coded, const void* base, unsig
 
 // The plain kernel: packed query rows of a segment, CTAs per SM.  The one for few rows (8 or 16 of them): warps of an SM that take shares.
 constexpr unsigned int kPagedPlainRows = 4, kPagedPlainCtas = 4, kPagedRowsWarps = 8;
+// Packed query rows of an entry up to which that one is taken.
+constexpr unsigned int kPagedFewRows = 16;
 
 // paged_rows.cu: a CTA on each of `sms` SMs; *per: its workers
 int launch_paged_rows(PagedParams& p, bool coded, unsigned int rows, unsigned int sms, unsigned int* per, cudaStream_t stream, bool pdl);
+
+// paged_tile.cu: a CTA on each SM; *piece_rows: packed query rows of a segment
+int launch_paged_tile(PagedParams& p, bool coded, unsigned int sms, unsigned int* piece_rows, cudaStream_t stream, bool pdl);
 
 }    // namespace b200

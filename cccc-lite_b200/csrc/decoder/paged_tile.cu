@@ -1,0 +1,627 @@
+// Attention of many query rows (prompts and their portions) over a cache in pages, tensor-bound, on tcgen05.
+//
+// A CTA on each SM takes its share of all segments' tiles.  A segment has RT times 128 packed query rows (a row is one query head of one
+// token), a tile KT keys.  The MMA lane issues S = Q K^T into tensor memory for 128 rows and sixty-four keys at a time; a warpgroup, one row per
+// thread, turns them into weights in the place of their scores; O += P V with P as the operand in tensor memory and V as it lies (an
+// MN-major operand).  As soon as a place's weights are in use the next tile's scores for it are issued, so that a warpgroup finds the
+// scores of one half of a tile ready while those of the other are made.
+// The running maximum only moves when it grows by more than 2^8, so that O is seldom rescaled.
+//
+// BF16 pages come by TMA (128-byte swizzle); rows that no query of the segment sees are cleared before the value product, since
+// 0 times what is no number is none.  E4M3 pages come through registers: four warps turn codes into the BF16 numbers that they stand
+// for, power of two included - exact, four significant bits - so that everything behind is the same for both.
+//
+// The weights are rounded to BF16 for the value product (2^-8 of each at most, half a step; their sum is kept in 32 bits): with the sum
+// of two BF16 numbers instead, the tensor cores have one and a half times the work.
+//
+// Every wait is bounded; on expiry the status word is raised, the roles drain, tensor memory is freed and the CTA returns.
+#include "paged_attention.cuh"
+#include "tile_common.cuh"
+
+#include <type_traits>
+
+namespace b200
+{
+
+template <int D, bool CODED>
+struct TileShape
+{
+    static constexpr int RT = D <= 128 ? 2 : 1;       // 128-row halves of a segment
+    static constexpr int KT = D <= 128 ? 128 : 64;    // keys of a tile
+    static constexpr int HALVES = KT / 64;
+    static constexpr int ROWS = 128 * RT;
+    static constexpr int LOADERS = CODED ? 7 : 1;     // warps
+    static constexpr int WARPS = 4 * RT + LOADERS + 1;
+    // E4M3 with two halves: 128 registers each at launch, then 136 for the two warpgroups of the rows and 120 for the others
+    static constexpr bool SPLIT = CODED && RT == 2;
+    static constexpr int QBLOCK = 128 * 128, BLOCK = KT * 128;    // bytes of 64 elements of 128 query rows, of KT keys
+    static constexpr int Q_BYTES = RT * (D / 64) * QBLOCK;
+    static constexpr int TILE = (D / 64) * BLOCK;
+    static constexpr int SMEM = 1024 + Q_BYTES + 4 * TILE + 1024;
+    // tensor memory: RT places of scores and weights, then RT outputs
+    static constexpr uint32_t S_COLS = KT, O_AT = RT * KT;
+    static constexpr uint32_t COLS = RT * (KT + D) <= 256 ? 256 : 512;
+};
+
+// An MN-major operand [k][64 elements] with the 128-byte swizzle: 8-k groups 1024 bytes apart, 64-element blocks `block` bytes apart.
+__device__ __forceinline__ uint64_t umma_desc_values(uint32_t smem_addr, uint32_t block)
+{
+    uint64_t d = 0;
+    d |= (uint64_t)((smem_addr & 0x3FFFFu) >> 4);
+    d |= (uint64_t)(block >> 4) << 16;
+    d |= (uint64_t)(1024 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+// Four codes times their row's power of two, as BF16 (exact).
+__device__ __forceinline__ uint2 e4m3x4_to_bf16(uint32_t four, float two)
+{
+    uint32_t a, b;
+    e4m3x4_to_f16x2(four, a, b);
+    const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&a)), y = __half22float2(*reinterpret_cast<const __half2*>(&b));
+    return make_uint2(pack_bf16x2(x.x * two, x.y * two), pack_bf16x2(y.x * two, y.y * two));
+}
+
+template <int D, bool CODED>
+__global__ void __launch_bounds__(32 * TileShape<D, CODED>::WARPS, 1) paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+    const __grid_constant__ PagedParams p, unsigned int box_rows, unsigned int* status)
+{
+    using S = TileShape<D, CODED>;
+    constexpr unsigned int KT = S::KT, ROWS = S::ROWS, RT = S::RT, THREADS = 32 * S::WARPS, INFOS = 4;
+    using Cursor = PagedCursor<KT, ROWS>;
+    extern __shared__ unsigned char pt_raw[];
+    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(pt_raw) + 1023) & ~(uintptr_t)1023);
+    __shared__ uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[RT][S::HALVES], p_ready[RT][S::HALVES], pv_done[RT], o_full[RT], q_ready[RT];
+    __shared__ unsigned int bad_s[INFOS];    // of a tile: sixteens of keys on no page
+    __shared__ PagedSums<THREADS> sums;
+    __shared__ uint32_t tmem_slot;
+    __shared__ volatile unsigned int abort_flag;
+    unsigned char *qs = smem, *ks = qs + S::Q_BYTES, *vs = ks + 2 * S::TILE;
+    const unsigned int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    constexpr unsigned int LOAD = 4 * RT, MMA = LOAD + S::LOADERS;    // first warps of the roles
+    if (threadIdx.x == 0)
+    {
+        for (int i = 0; i < 2; i++)
+        {
+            mbar_init(k_full + i, S::LOADERS);
+            mbar_init(v_full + i, S::LOADERS);
+            mbar_init(k_empty + i, 1);
+            mbar_init(v_empty + i, 1);
+        }
+        for (unsigned int x = 0; x < RT; x++)
+        {
+            mbar_init(pv_done + x, 1);
+            mbar_init(o_full + x, 1);
+            mbar_init(q_ready + x, 4);
+            for (int h = 0; h < S::HALVES; h++) 
+            {
+                mbar_init(&s_full[x][h], 1);
+                mbar_init(&p_ready[x][h], 4);
+            }
+        }
+        abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == MMA) { tmem_alloc(&tmem_slot, S::COLS); }
+    grid_dependency_launch();
+    grid_dependency_wait();
+    tc_fence_before();
+    paged_sums<KT, ROWS, THREADS>(p, &sums);    // (its barriers stand behind what is set up above)
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    const PagedShare share = paged_share<KT, ROWS, THREADS>(p, sums, blockIdx.x, gridDim.x);
+    const unsigned int length = (unsigned int)(share.end - share.begin);
+    if (threadIdx.x == 0) { p.header[blockIdx.x] = PagedHeader{}; }    // (a segment left unfinished is noted by the same thread)
+    auto wait = [&](uint64_t* bar, unsigned int parity) { return abort_flag == 0 && mbar_wait_bounded(bar, parity & 1u); };
+    auto give_up = [&](unsigned int role, unsigned int step) {
+        note_timeout(status, WAIT_PAGED_TILE, role, step);
+        abort_flag = 1;
+    };
+    Cursor cur;
+    if (length != 0) { cur.at(p, share); }
+
+    if constexpr (S::SPLIT)
+    {
+        if (warp < LOAD) { asm volatile("setmaxnreg.inc.sync.aligned.u32 136;"); }
+        else { asm volatile("setmaxnreg.dec.sync.aligned.u32 120;"); }
+    }
+    if (length == 0) {}
+    else if (warp >= LOAD && warp < MMA)
+    {
+        unsigned int tile = 0;    // of the share
+        bool ok = true;
+        if constexpr (!CODED)
+        {
+            // lane i asks for the i-th box of rows (a page, or a tile's part of one)
+            const unsigned int boxes = KT / box_rows;
+            for (unsigned int at = 0; at < length && ok;)
+            {
+                const unsigned int units = cur.take(length - at);
+                auto page_of = [&](unsigned int i) {
+                    const unsigned int key = cur.s.unit(cur.unit + i) * KT + lane * box_rows;
+                    const bool meets = lane < boxes && key < cur.s.lim && (key + box_rows > cur.s.low || (key + box_rows > cur.v.floor && key < cur.s.first_end));
+                    return meets ? p.c.table[(size_t)(unsigned int)cur.v.slot * p.c.ld_table + (key >> p.c.shift)] : -1;
+                };
+                int next = page_of(0);
+                for (unsigned int i = 0; i < units; i++, tile++)
+                {
+                    const unsigned int st = tile & 1u, key = cur.s.unit(cur.unit + i) * KT + lane * box_rows;
+                    const bool none = (unsigned int)next >= p.c.pages;
+                    const int z = none ? (int)p.c.pages : next;    // behind the caches' end: zeros
+                    const int row = (int)((cur.kvh << p.c.shift) + (key & ((1u << p.c.shift) - 1u)));
+                    unsigned int bad = __ballot_sync(0xFFFFFFFFu, lane < boxes && none);
+                    if (i + 1 < units) { next = page_of(i + 1); }
+                    ok = tile < 2 || __all_sync(0xFFFFFFFFu, wait(k_empty + st, (tile >> 1) - 1));
+                    if (!ok) { break; }
+                    if (lane == 0)
+                    {
+                        unsigned int wide = 0;    // a bit for every sixteen keys
+                        for (unsigned int b = 0; b < boxes; b++) { wide |= (bad >> b & 1u) ? ((1u << (box_rows / 16)) - 1u) << (b * (box_rows / 16)) : 0u; }
+                        bad_s[tile % INFOS] = wide;
+                        mbar_expect_tx(k_full + st, S::TILE);
+                    }
+                    __syncwarp();
+                    if (lane < boxes)
+                    {
+#pragma unroll
+                        for (int b = 0; b < D / 64; b++) { tma_load_3d(ks + st * S::TILE + b * S::BLOCK + lane * box_rows * 128, &tmK, b * 64, row, z, k_full + st); }
+                    }
+                    __syncwarp();
+                    if (lane == 0) { mbar_arrive(k_full + st); }
+                    ok = tile < 2 || __all_sync(0xFFFFFFFFu, wait(v_empty + st, (tile >> 1) - 1));
+                    if (!ok) { break; }
+                    if (lane == 0) { mbar_expect_tx(v_full + st, S::TILE); }
+                    __syncwarp();
+                    if (lane < boxes)
+                    {
+#pragma unroll
+                        for (int b = 0; b < D / 64; b++) { tma_load_3d(vs + st * S::TILE + b * S::BLOCK + lane * box_rows * 128, &tmV, b * 64, row, z, v_full + st); }
+                    }
+                    __syncwarp();
+                    if (lane == 0) { mbar_arrive(v_full + st); }
+                }
+                at += units;
+                if (at < length) { cur.next(p); }
+            }
+            if (!ok && lane == 0) { give_up(0, tile); }
+            // the copies in flight arrive (bounded) before the CTA may leave
+            if (lane == 0)
+            {
+                for (unsigned int j = tile < 2 ? 0 : tile - 2; j < tile; j++)
+                {
+                    mbar_wait_bounded(k_full + (j & 1u), (j >> 1) & 1u);
+                    mbar_wait_bounded(v_full + (j & 1u), (j >> 1) & 1u);
+                }
+                if (!ok && tile >= 2) { mbar_wait_bounded(k_full + (tile & 1u), (tile >> 1) & 1u); }
+            }
+        }
+        else
+        {
+            // LPR lanes a row, sixteen codes each; the warps take a tile's groups of PER rows in turn, keys and then values (with them from where
+            // the keys have left off).  The next tile's rows are under way while this one's are turned into numbers.
+            constexpr unsigned int LPR = D / 16, PER = 32 / LPR, GROUPS = KT / PER, MOST = (GROUPS + S::LOADERS - 1) / S::LOADERS;
+            const unsigned int c = lane % LPR, r = lane / LPR, w = warp - LOAD;
+            const unsigned int first[2] = { w, (w + S::LOADERS - GROUPS % S::LOADERS) % S::LOADERS };
+            uint4 raw[2][MOST];
+            unsigned int two[2][MOST];
+            int sixteen = 0;    // the page of the lane's sixteen keys of the tile
+            unsigned int i = 0, at = 0, units = cur.take(length);    // the tile that is fetched next: of its segment; where that begins in the share
+            auto fetch = [&](int which) {
+                const unsigned int key0 = cur.s.unit(cur.unit + i) * KT, ld = which ? p.c.v_ld : p.c.k_ld;
+                const unsigned char *x = which ? p.c.v : p.c.k, *scale = which ? p.c.v_scale : p.c.k_scale;
+                const int* table = p.c.table + (size_t)(unsigned int)cur.v.slot * p.c.ld_table;    // (looked at for a wanted key only)
+                int page[MOST];
+#pragma unroll
+                for (unsigned int a = 0; a < MOST; a++)
+                {
+                    const unsigned int group = first[which] + a * S::LOADERS, key = key0 + group * PER + r;
+                    page[a] = group < GROUPS && paged_wanted(cur.v, cur.s, key) ? table[key >> p.c.shift] : -1;
+                }
+                if (which == 0)
+                {
+                    const unsigned int key = key0 + lane * 16;
+                    const bool meets = lane < KT / 16 && key < cur.s.lim && (key + 16 > cur.s.low || (key + 16 > cur.v.floor && key < cur.s.first_end));
+                    sixteen = meets ? table[key >> p.c.shift] : 0;
+                }
+#pragma unroll
+                for (unsigned int a = 0; a < MOST; a++)
+                {
+                    const unsigned int key = key0 + (first[which] + a * S::LOADERS) * PER + r;
+                    const bool have = (unsigned int)page[a] < p.c.pages;
+                    const size_t row = have ? paged_row(p.c, page[a], cur.kvh, key) : 0;
+                    raw[which][a] = have && c * 16 < ld ? *reinterpret_cast<const uint4*>(x + row * ld + c * 16) : make_uint4(0, 0, 0, 0);
+                    two[which][a] = have ? scale[row] : 0u;
+                }
+            };
+            auto store = [&](int which, unsigned char* to) {
+#pragma unroll
+                for (unsigned int a = 0; a < MOST; a++)
+                {
+                    const unsigned int group = first[which] + a * S::LOADERS, row = group * PER + r;
+                    if (group >= GROUPS) { break; }
+                    const float f = paged_two(two[which][a]);
+                    const uint4 u = raw[which][a];
+                    const uint2 x0 = e4m3x4_to_bf16(u.x, f), x1 = e4m3x4_to_bf16(u.y, f), x2 = e4m3x4_to_bf16(u.z, f), x3 = e4m3x4_to_bf16(u.w, f);
+                    const uint32_t base = smem_u32(to) + (c / 4) * S::BLOCK + row * 128, p0 = (((c % 4) * 2) ^ (row & 7u)) * 16, p1 = p0 ^ 16;
+                    // the lanes of every other block begin with their second piece: no two meet in a bank
+                    const bool turn = ((c / 4) & 1u) != 0;
+                    sts128(base + (turn ? p1 : p0), turn ? x2.x : x0.x, turn ? x2.y : x0.y, turn ? x3.x : x1.x, turn ? x3.y : x1.y);
+                    sts128(base + (turn ? p0 : p1), turn ? x0.x : x2.x, turn ? x0.y : x2.y, turn ? x1.x : x3.x, turn ? x1.y : x3.y);
+                }
+                fence_proxy_async();
+                __syncwarp();
+            };
+            fetch(0);
+            for (; tile < length && ok; tile++)
+            {
+                const unsigned int st = tile & 1u;
+                fetch(1);
+                ok = tile < 2 || __all_sync(0xFFFFFFFFu, wait(k_empty + st, (tile >> 1) - 1));
+                if (!ok) { break; }
+                const unsigned int bad = __ballot_sync(0xFFFFFFFFu, (unsigned int)sixteen >= p.c.pages);
+                if (w == 0 && lane == 0) { bad_s[tile % INFOS] = bad; }
+                store(0, ks + st * S::TILE);
+                if (lane == 0) { mbar_arrive(k_full + st); }
+                if (++i == units)
+                {
+                    at += units;
+                    i = 0;
+                    if (at < length)
+                    {
+                        cur.next(p);
+                        units = cur.take(length - at);
+                    }
+                }
+                if (tile + 1 < length) { fetch(0); }
+                ok = tile < 2 || __all_sync(0xFFFFFFFFu, wait(v_empty + st, (tile >> 1) - 1));
+                if (!ok) { break; }
+                store(1, vs + st * S::TILE);
+                if (lane == 0) { mbar_arrive(v_full + st); }
+            }
+            if (!ok && lane == 0) { give_up(0, tile); }
+        }
+    }
+    else if (warp == MMA)
+    {
+        const uint32_t idesc_s = umma_idesc_bf16(128, 64), idesc_o = umma_idesc_bf16(128, D) | (1u << 16);    // V is MN-major
+        // (adding n >> 4 to a descriptor moves it on by n bytes)
+        const uint64_t q_desc = umma_desc_kmajor_sw128(smem_u32(qs)), k_desc = umma_desc_kmajor_sw128(smem_u32(ks)), v_desc = umma_desc_values(smem_u32(vs), S::BLOCK);
+        unsigned int tile = 0, queries[RT] = {}, weights[RT] = {};    // tiles taken; of each half of the rows: segments, tiles whose weights were waited for
+        bool ok = true;
+        for (unsigned int at = 0; at < length && ok;)
+        {
+            const unsigned int units = cur.take(length - at), halves = cur.s.rows > 128 ? RT : 1;
+            // sixty-four keys of tile j against one half of the rows
+            auto scores = [&](unsigned int x, unsigned int j, unsigned int h) {
+                if (elect_one())
+                {
+                    const uint64_t q = q_desc + x * (D / 64) * (S::QBLOCK >> 4), kd = k_desc + (j & 1u) * (S::TILE >> 4) + h * (64 * 128 >> 4);
+                    const uint32_t to = tmem + x * S::S_COLS + h * 64;
+#pragma unroll
+                    for (int k = 0; k < D / 16; k++)
+                    {
+                        if (k * 16 < (int)p.c.dim)
+                        {
+                            umma_bf16(to, q + (k / 4) * (S::QBLOCK >> 4) + (k % 4) * 2, kd + (k / 4) * (S::BLOCK >> 4) + (k % 4) * 2, idesc_s, k != 0 ? 1u : 0u);
+                        }
+                    }
+                    if (x + 1 == halves && h + 1 == S::HALVES) { umma_commit(k_empty + (j & 1u)); }
+                    umma_commit(&s_full[x][h]);
+                }
+                __syncwarp();
+            };
+            ok = wait(k_full + (tile & 1u), tile >> 1);
+#pragma unroll
+            for (unsigned int x = 0; x < RT; x++)
+            {
+                if (x >= halves || !ok) { break; }
+                ok = wait(q_ready + x, queries[x]++);
+                tc_fence_after();
+                for (unsigned int h = 0; ok && h < S::HALVES; h++) { scores(x, tile, h); }
+            }
+            for (unsigned int i = 0; i < units && ok; i++, tile++)
+            {
+                const unsigned int st = tile & 1u;
+                ok = wait(v_full + st, tile >> 1);
+                if (!ok) { break; }
+                tc_fence_after();
+                if constexpr (!CODED)
+                {
+                    const unsigned int key0 = cur.s.unit(cur.unit + i) * KT;
+                    if (key0 < cur.s.low || key0 + KT > cur.s.lim)
+                    {
+                        // rows that nobody sees may hold anything
+                        for (unsigned int j = lane; j < KT; j += 32)
+                        {
+                            if (paged_wanted(cur.v, cur.s, key0 + j)) { continue; }
+#pragma unroll
+                            for (int b = 0; b < D / 64; b++)
+                            {
+#pragma unroll
+                                for (int k = 0; k < 8; k++) { sts128(smem_u32(vs) + st * S::TILE + b * S::BLOCK + j * 128 + k * 16, 0, 0, 0, 0); }
+                            }
+                        }
+                        fence_proxy_async();
+                        __syncwarp();
+                    }
+                }
+#pragma unroll 1
+                for (unsigned int h = 0; h < S::HALVES; h++)
+                {
+#pragma unroll
+                    for (unsigned int x = 0; x < RT; x++)
+                    {
+                        if (x >= halves || !ok) { break; }
+                        ok = wait(&p_ready[x][h], weights[x]);
+                        if (!ok) { break; }
+                        tc_fence_after();
+                        if (elect_one())
+                        {
+                            const uint64_t vd = v_desc + st * (S::TILE >> 4) + h * (4 * 2048 >> 4);
+#pragma unroll
+                            for (int k = 0; k < 4; k++)
+                            {
+                                umma_bf16_ts(tmem + S::O_AT + x * D, tmem + x * S::S_COLS + h * 64 + k * 8, vd + k * (2048 >> 4), idesc_o, (i | h | (unsigned int)k) != 0 ? 1u : 0u);
+                            }
+                            umma_commit(pv_done + x);
+                            if (h + 1 == S::HALVES)
+                            {
+                                if (x + 1 == halves) { umma_commit(v_empty + st); }
+                                if (i + 1 == units) { umma_commit(o_full + x); }
+                            }
+                        }
+                        __syncwarp();
+                        if (h + 1 == S::HALVES) { weights[x]++; }
+                        // into the place of the weights just issued: products of one thread run in the order of their issue
+                        if (i + 1 < units)
+                        {
+                            if (x == 0 && h == 0)
+                            {
+                                ok = wait(k_full + ((tile + 1) & 1u), (tile + 1) >> 1);
+                                if (!ok) { break; }
+                                tc_fence_after();
+                            }
+                            scores(x, tile + 1, h);
+                        }
+                    }
+                }
+            }
+            at += units;
+            if (at < length) { cur.next(p); }
+        }
+        if (!ok)
+        {
+            if (lane == 0) { give_up(1, tile); }
+            if (elect_one()) { umma_commit(pv_done); }    // completes once the products in flight have stopped reading shared memory
+            __syncwarp();
+        }
+    }
+    else
+    {
+        const unsigned int x = warp / 4, quarter = warp & 3u, rl = quarter * 32 + lane;
+        const uint32_t place = tmem + ((quarter * 32u) << 16) + x * S::S_COLS, o_at = tmem + ((quarter * 32u) << 16) + S::O_AT + x * D;
+        const float scale2 = fmaxf(fabsf(p.scale) * 1.44269504088896341f, 1e-30f);    // 0 times a masked -inf would be no number
+        const bool vec_q = (p.c.dim % 8) == 0 && (p.ldq % 8) == 0 && (reinterpret_cast<uintptr_t>(p.q) % 16) == 0;
+        const bool vec_o = (p.c.vdim % 8) == 0 && (p.ldo % 8) == 0 && (reinterpret_cast<uintptr_t>(p.out) % 16) == 0;
+        const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;    // the maximum is taken before scaling
+        const unsigned int VL = paged_ld(p.c.vdim);
+        unsigned int tile = 0, scored = 0, weighted = 0, outputs = 0;    // tiles; this half of the rows' tiles, their halves, outputs
+        bool ok = true;
+        for (unsigned int at = 0; at < length && ok;)
+        {
+            const unsigned int units = cur.take(length - at);
+            const PagedEntry& v = cur.v;
+            const PagedSegment& s = cur.s;
+            const bool active = x == 0 || s.rows > 128;
+            const unsigned int i_row = x * 128 + rl, r = s.r0 + i_row;
+            const bool real = i_row < s.rows;
+            const unsigned int t = v.pos + (real ? r / p.G : 0), tok = v.start + (real ? r / p.G : 0), head = cur.kvh * p.G + (real ? r % p.G : 0);
+            if (active)
+            {
+                const __nv_bfloat16* src = (const __nv_bfloat16*)p.q + (size_t)tok * p.ldq + (size_t)head * p.c.dim;
+#pragma unroll 16
+                for (int c = 0; c < D / 8; c++)
+                {
+                    uint4 u = make_uint4(0, 0, 0, 0);
+                    if (real && c * 8 < (int)p.c.dim)
+                    {
+                        if (vec_q) { u = *reinterpret_cast<const uint4*>(src + c * 8); }
+                        else
+                        {
+                            uint32_t w[8];
+#pragma unroll
+                            for (int j = 0; j < 8; j++) { w[j] = c * 8 + j < (int)p.c.dim ? __bfloat16_as_ushort(src[c * 8 + j]) : 0u; }
+                            u = make_uint4(w[0] | (w[1] << 16), w[2] | (w[3] << 16), w[4] | (w[5] << 16), w[6] | (w[7] << 16));
+                        }
+                    }
+                    sts128(smem_u32(qs) + (x * (D / 64) + c / 8) * S::QBLOCK + rl * 128 + (((c % 8) ^ (rl & 7u)) * 16), u.x ^ flip, u.y ^ flip, u.z ^ flip, u.w ^ flip);
+                }
+                fence_proxy_async();
+                tc_fence_before();    // the last segment's outputs have been read before this one's products
+                __syncwarp();
+                if (lane == 0) { mbar_arrive(q_ready + x); }
+                // keys of the row: low .. lim - 1 and floor .. first_end - 1
+                const unsigned int lim = real ? min(t + 1, s.lim) : 0u, low = max(v.floor, p.window != 0 && t + 1 > p.window ? t + 1 - p.window : 0u);
+                const unsigned int first_end = s.first_end;
+                // keys that every row of this half sees
+                const unsigned int last_row = s.r0 + min(s.rows, x * 128 + 128) - 1, t_last = v.pos + last_row / p.G;
+                const unsigned int lim_all = min(v.pos + (s.r0 + x * 128) / p.G + 1, s.lim);
+                const unsigned int low_all = max(v.floor, p.window != 0 && t_last + 1 > p.window ? t_last + 1 - p.window : 0u);
+                float m = -INFINITY, l = 0.f;
+                for (unsigned int i = 0; i < units && ok; i++)
+                {
+                    const unsigned int key0 = s.unit(cur.unit + i) * KT;
+#pragma unroll
+                    for (int h = 0; h < S::HALVES; h++)
+                    {
+                        ok = __all_sync(0xFFFFFFFFu, wait(&s_full[x][h], scored));
+                        if (!ok) { break; }
+                        tc_fence_after();
+                        uint32_t z[64];
+                        tmem_ld_32x32(place + h * 64, *reinterpret_cast<uint32_t(*)[32]>(z));
+                        tmem_ld_32x32(place + h * 64 + 32, *reinterpret_cast<uint32_t(*)[32]>(z + 32));
+                        tmem_ld_wait();
+                        const unsigned int k0 = key0 + h * 64, bad = bad_s[(tile + i) % INFOS] >> (h * 4) & 15u;
+                        if (bad != 0 || k0 < low_all || k0 + 64 > lim_all)
+                        {
+                            // the keys that the row sees, a bit each
+                            auto below = [&](unsigned int key) { return key <= k0 ? 0ull : key - k0 >= 64 ? ~0ull : (1ull << (key - k0)) - 1ull; };
+                            unsigned long long seen = below(lim) & (~below(low) | (below(first_end) & ~below(v.floor)));
+#pragma unroll
+                            for (int b = 0; b < 4; b++) { seen &= (bad >> b & 1u) ? ~(0xFFFFull << (16 * b)) : ~0ull; }
+                            const uint32_t w[2] = { (uint32_t)seen, (uint32_t)(seen >> 32) };
+#pragma unroll
+                            for (int j = 0; j < 64; j++) { z[j] = (w[j / 32] >> (j % 32) & 1u) != 0 ? z[j] : 0xFF800000u; }    // else -inf
+                        }
+                        float mx[4] = { -INFINITY, -INFINITY, -INFINITY, -INFINITY };    // four maxima in flight
+#pragma unroll
+                        for (int j = 0; j < 64; j++) { mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(z[j])); }
+                        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale2;
+                        float c = 1.f;
+                        if (top > m + 8.f)
+                        {
+                            c = exp2_f32(m - top);    // 0 where nothing came before
+                            m = top;
+                            l *= c;
+                        }
+                        const float base = m == -INFINITY ? 0.f : m;
+                        uint32_t w[32];
+                        float sum[2] = { 0.f, 0.f };
+#pragma unroll
+                        for (int j = 0; j < 32; j++)
+                        {
+                            const float a = exp2_f32(fmaf(__uint_as_float(z[2 * j]), scale2, -base)), b = exp2_f32(fmaf(__uint_as_float(z[2 * j + 1]), scale2, -base));
+                            sum[0] += a;
+                            sum[1] += b;
+                            w[j] = pack_bf16x2(a, b);
+                        }
+                        l += sum[0] + sum[1];
+                        if ((i | (unsigned int)h) != 0 && __any_sync(0xFFFFFFFFu, c != 1.f))
+                        {
+                            // the products before leave O alone; the next one waits for these weights
+                            ok = __all_sync(0xFFFFFFFFu, wait(pv_done + x, weighted - 1));
+                            if (!ok) { break; }
+                            tc_fence_after();
+#pragma unroll
+                            for (int d = 0; d < D; d += 32)
+                            {
+                                uint32_t o[32];
+                                tmem_ld_32x32(o_at + d, o);
+                                tmem_ld_wait();
+#pragma unroll
+                                for (int j = 0; j < 32; j++) { o[j] = __float_as_uint(__uint_as_float(o[j]) * c); }
+                                tmem_st_32x16(o_at + d, o);
+                                tmem_st_32x16(o_at + d + 16, o + 16);
+                            }
+                        }
+                        tmem_st_32x16(place + h * 64, w);
+                        tmem_st_32x16(place + h * 64 + 16, w + 16);
+                        tmem_st_wait();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) { mbar_arrive(&p_ready[x][h]); }
+                        weighted++;
+                    }
+                    scored++;
+                }
+                ok = ok && __all_sync(0xFFFFFFFFu, wait(o_full + x, outputs));
+                if (!ok) { break; }
+                outputs++;
+                tc_fence_after();
+                const bool whole = cur.whole(units);
+                float* piece = p.partial + (2 * (size_t)blockIdx.x + (cur.unit == 0 ? 1 : 0)) * paged_piece(ROWS, p.c.vdim);
+                const float f = whole ? paged_factor(p, head, m, l) : 1.f;
+                __nv_bfloat16* out = (__nv_bfloat16*)p.out + (size_t)tok * p.ldo + (size_t)head * p.c.vdim;
+#pragma unroll
+                for (int d = 0; d < D; d += 32)
+                {
+                    if (d >= (int)p.c.vdim) { break; }
+                    uint32_t o[32];
+                    tmem_ld_32x32(o_at + d, o);
+                    tmem_ld_wait();
+                    if (real)
+                    {
+#pragma unroll
+                        for (int q = 0; q < 32; q += 8)
+                        {
+                            float y[8];
+#pragma unroll
+                            for (int j = 0; j < 8; j++) { y[j] = __uint_as_float(o[q + j]) * f; }
+                            if (!whole)
+                            {
+                                if (d + q < (int)VL)
+                                {
+                                    store4(piece + (size_t)i_row * VL + d + q, make_float4(y[0], y[1], y[2], y[3]));
+                                    store4(piece + (size_t)i_row * VL + d + q + 4, make_float4(y[4], y[5], y[6], y[7]));
+                                }
+                            }
+                            else if (vec_o)
+                            {
+                                if (d + q < (int)p.c.vdim)
+                                {
+                                    *reinterpret_cast<uint4*>(out + d + q) =
+                                        make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]), pack_bf16x2(y[6], y[7]));
+                                }
+                            }
+                            else
+                            {
+#pragma unroll
+                                for (int j = 0; j < 8; j++)
+                                {
+                                    if (d + q + j < (int)p.c.vdim) { out[d + q + j] = __float2bfloat16_rn(y[j]); }
+                                }
+                            }
+                        }
+                    }
+                    __syncwarp();
+                }
+                if (real && !whole)
+                {
+                    piece[ROWS * VL + i_row] = m;
+                    piece[ROWS * VL + ROWS + i_row] = l;
+                }
+            }
+            if (threadIdx.x == 0 && cur.unit == 0 && !cur.whole(units))
+            {
+                p.header[blockIdx.x] = PagedHeader{ cur.last(share, share.begin + at) - blockIdx.x + 1, blockIdx.x, s.rows, s.r0, v.start, cur.kvh };
+            }
+            tile += units;
+            at += units;
+            if (at < length) { cur.next(p); }
+        }
+        if (!ok && lane == 0) { give_up(2 + x, tile); }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == MMA) { tmem_dealloc(tmem, S::COLS); }
+}
+
+template <int D, bool CODED>
+static int run_tile(PagedParams& p, unsigned int sms, unsigned int* piece_rows, cudaStream_t stream, bool pdl)
+{
+    using S = TileShape<D, CODED>;
+    p.least = 2;
+    *piece_rows = S::ROWS;
+    unsigned int* status = decoder_status_word();
+    if (!status) { return 1; }
+    const unsigned int page = 1u << p.c.shift, box = page < (unsigned int)S::KT ? page : (unsigned int)S::KT;
+    CUtensorMap tk, tv;
+    memset(&tk, 0, sizeof(tk));
+    memset(&tv, 0, sizeof(tv));
+    if (!CODED && (!make_paged_map(&tk, false, p.c.k, p.c.k_ld, p.c, 64, box, true) || !make_paged_map(&tv, false, p.c.v, p.c.v_ld, p.c, 64, box, true))) { return -1; }
+    return launch_kernel("paged_tile", paged_tile_kernel<D, CODED>, dim3(sms), dim3(32 * S::WARPS), (size_t)S::SMEM, stream, pdl, tk, tv, p, box, status);
+}
+
+int launch_paged_tile(PagedParams& p, bool coded, unsigned int sms, unsigned int* piece_rows, cudaStream_t stream, bool pdl)
+{
+    const unsigned int width = p.c.dim > p.c.vdim ? p.c.dim : p.c.vdim;
+    auto by_width = [&](auto c) {
+        constexpr bool CODED = decltype(c)::value;
+        return width <= 64 ? run_tile<64, CODED>(p, sms, piece_rows, stream, pdl) : width <= 128 ? run_tile<128, CODED>(p, sms, piece_rows, stream, pdl)
+                                                                                                 : run_tile<256, CODED>(p, sms, piece_rows, stream, pdl);
+    };
+    return coded ? by_width(std::true_type()) : by_width(std::false_type());
+}
+
+}    // namespace b200

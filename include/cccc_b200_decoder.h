@@ -188,7 +188,8 @@ typedef struct cuda_b200_paged_attention
 } cuda_b200_paged_attention;
 /* Bytes of scratch on the current device for calls of up to max_n tokens per entry (0 for sizes that are not taken). */
 C_EXPORT unsigned long long cuda_b200_paged_attention_work_bytes(unsigned int H, unsigned int Hkv, unsigned int vdim, unsigned int max_n);
-/* kernel: 0 = by shape, 1 = the plain kernel (always in float mode), 2 = for few query rows, on mma.sync (BF16). */
+/* kernel: 0 = by shape, 1 = the plain kernel (always in float mode), 2 = for few query rows, on
+ * mma.sync, 3 = for many, on tcgen05 (both BF16; their weights enter the value product as described there). */
 C_EXPORT int cuda_b200_paged_attention_rows(int dtype, const cuda_b200_paged_attention* a, const cuda_b200_pages* c, const cuda_b200_batch* b, void* stream,
     unsigned int flags, int kernel);
 
