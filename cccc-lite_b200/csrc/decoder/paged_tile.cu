@@ -30,30 +30,20 @@ struct TileShape
     static constexpr int KT = D <= 128 ? 128 : 64;    // keys of a tile
     static constexpr int HALVES = KT / 64;
     static constexpr int ROWS = 128 * RT;
-    static constexpr int LOADERS = CODED ? 7 : 1;     // warps
-    static constexpr int WARPS = 4 * RT + LOADERS + 1;
+    static constexpr int LOADERS = CODED ? 8 - RT : 1;    // warps
+    static constexpr int WARPS = 4 * RT + LOADERS + RT;   // a warpgroup and an issuing warp for each half of the rows
     // E4M3 with two halves: 128 registers each at launch, then 136 for the two warpgroups of the rows and 120 for the others
     static constexpr bool SPLIT = CODED && RT == 2;
-    static constexpr int QBLOCK = 128 * 128, BLOCK = KT * 128;    // bytes of 64 elements of 128 query rows, of KT keys
+    static constexpr int QBLOCK = 128 * 128, BLOCK = 64 * 128;    // bytes of 64 elements of 128 query rows, of 64 keys
     static constexpr int Q_BYTES = RT * (D / 64) * QBLOCK;
-    static constexpr int TILE = (D / 64) * BLOCK;
-    static constexpr int SMEM = 1024 + Q_BYTES + 4 * TILE + 1024;
+    static constexpr int STAGE = (D / 64) * BLOCK;    // 64 keys, or their values
+    static constexpr int STAGES = D <= 128 ? 4 : 2;
+    static constexpr int SMEM = 1024 + Q_BYTES + 2 * STAGES * STAGE + 1024;
     // tensor memory: RT places of scores and weights, then RT outputs
     static constexpr uint32_t S_COLS = KT, O_AT = RT * KT;
     static constexpr uint32_t COLS = RT * (KT + D) <= 256 ? 256 : 512;
 };
 
-// An MN-major operand [k][64 elements] with the 128-byte swizzle: 8-k groups 1024 bytes apart, 64-element blocks `block` bytes apart.
-__device__ __forceinline__ uint64_t umma_desc_values(uint32_t smem_addr, uint32_t block)
-{
-    uint64_t d = 0;
-    d |= (uint64_t)((smem_addr & 0x3FFFFu) >> 4);
-    d |= (uint64_t)(block >> 4) << 16;
-    d |= (uint64_t)(1024 >> 4) << 32;
-    d |= (uint64_t)1 << 46;
-    d |= (uint64_t)2 << 61;
-    return d;
-}
 // Four codes times their row's power of two, as BF16 (exact).
 __device__ __forceinline__ uint2 e4m3x4_to_bf16(uint32_t four, float two)
 {
@@ -68,33 +58,33 @@ __global__ void __launch_bounds__(32 * TileShape<D, CODED>::WARPS, 1) paged_tile
     const __grid_constant__ PagedParams p, unsigned int box_rows, unsigned int* status)
 {
     using S = TileShape<D, CODED>;
-    constexpr unsigned int KT = S::KT, ROWS = S::ROWS, RT = S::RT, THREADS = 32 * S::WARPS, INFOS = 4;
+    constexpr unsigned int KT = S::KT, ROWS = S::ROWS, RT = S::RT, THREADS = 32 * S::WARPS, INFOS = 8, HALVES = S::HALVES, NS = S::STAGES;
     using Cursor = PagedCursor<KT, ROWS>;
     extern __shared__ unsigned char pt_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(pt_raw) + 1023) & ~(uintptr_t)1023);
-    __shared__ uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[RT][S::HALVES], p_ready[RT][S::HALVES], pv_done[RT], o_full[RT], q_ready[RT];
-    __shared__ unsigned int bad_s[INFOS];    // of a tile: sixteens of keys on no page
+    __shared__ uint64_t k_full[NS], k_empty[NS], v_full[NS], v_empty[NS], s_full[RT][S::HALVES], p_ready[RT][S::HALVES], pv_done[RT], o_full[RT], q_ready[RT];
+    __shared__ unsigned int bad_s[INFOS];    // of 64 keys: sixteens on no page
     __shared__ PagedSums<THREADS> sums;
     __shared__ uint32_t tmem_slot;
     __shared__ volatile unsigned int abort_flag;
-    unsigned char *qs = smem, *ks = qs + S::Q_BYTES, *vs = ks + 2 * S::TILE;
+    unsigned char *qs = smem, *ks = qs + S::Q_BYTES, *vs = ks + NS * S::STAGE;
     const unsigned int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     constexpr unsigned int LOAD = 4 * RT, MMA = LOAD + S::LOADERS;    // first warps of the roles
     if (threadIdx.x == 0)
     {
-        for (int i = 0; i < 2; i++)
+        for (unsigned int i = 0; i < NS; i++)
         {
             mbar_init(k_full + i, S::LOADERS);
             mbar_init(v_full + i, S::LOADERS);
-            mbar_init(k_empty + i, 1);
-            mbar_init(v_empty + i, 1);
+            mbar_init(k_empty + i, RT);
+            mbar_init(v_empty + i, RT);
         }
         for (unsigned int x = 0; x < RT; x++)
         {
             mbar_init(pv_done + x, 1);
             mbar_init(o_full + x, 1);
             mbar_init(q_ready + x, 4);
-            for (int h = 0; h < S::HALVES; h++) 
+            for (int h = 0; h < HALVES; h++) 
             {
                 mbar_init(&s_full[x][h], 1);
                 mbar_init(&p_ready[x][h], 4);
@@ -113,7 +103,7 @@ __global__ void __launch_bounds__(32 * TileShape<D, CODED>::WARPS, 1) paged_tile
     const PagedShare share = paged_share<KT, ROWS, THREADS>(p, sums, blockIdx.x, gridDim.x);
     const unsigned int length = (unsigned int)(share.end - share.begin);
     if (threadIdx.x == 0) { p.header[blockIdx.x] = PagedHeader{}; }    // (a segment left unfinished is noted by the same thread)
-    auto wait = [&](uint64_t* bar, unsigned int parity) { return abort_flag == 0 && mbar_wait_bounded(bar, parity & 1u); };
+    auto wait = [&](uint64_t* bar, unsigned int parity) { return mbar_try_wait(bar, parity & 1u) || (abort_flag == 0 && mbar_wait_bounded(bar, parity & 1u)); };
     auto give_up = [&](unsigned int role, unsigned int step) {
         note_timeout(status, WAIT_PAGED_TILE, role, step);
         abort_flag = 1;
@@ -129,107 +119,122 @@ __global__ void __launch_bounds__(32 * TileShape<D, CODED>::WARPS, 1) paged_tile
     if (length == 0) {}
     else if (warp >= LOAD && warp < MMA)
     {
-        unsigned int tile = 0;    // of the share
+        unsigned int n = 0;    // stages filled
         bool ok = true;
         if constexpr (!CODED)
         {
-            // lane i asks for the i-th box of rows (a page, or a tile's part of one)
-            const unsigned int boxes = KT / box_rows;
+            // lane i asks for the i-th box of rows (a page, or a stage's part of one)
+            const unsigned int boxes = 64 / box_rows;
             for (unsigned int at = 0; at < length && ok;)
             {
-                const unsigned int units = cur.take(length - at);
+                const unsigned int units = cur.take(length - at) * HALVES;    // stages of the segment's part
+                auto key_of = [&](unsigned int i) { return cur.s.unit(cur.unit + i / HALVES) * KT + i % HALVES * 64 + lane * box_rows; };
                 auto page_of = [&](unsigned int i) {
-                    const unsigned int key = cur.s.unit(cur.unit + i) * KT + lane * box_rows;
+                    const unsigned int key = key_of(i);
                     const bool meets = lane < boxes && key < cur.s.lim && (key + box_rows > cur.s.low || (key + box_rows > cur.v.floor && key < cur.s.first_end));
                     return meets ? p.c.table[(size_t)(unsigned int)cur.v.slot * p.c.ld_table + (key >> p.c.shift)] : -1;
                 };
                 int next = page_of(0);
-                for (unsigned int i = 0; i < units; i++, tile++)
+                for (unsigned int i = 0; i < units; i++, n++)
                 {
-                    const unsigned int st = tile & 1u, key = cur.s.unit(cur.unit + i) * KT + lane * box_rows;
+                    const unsigned int st = n % NS, key = key_of(i);
                     const bool none = (unsigned int)next >= p.c.pages;
                     const int z = none ? (int)p.c.pages : next;    // behind the caches' end: zeros
                     const int row = (int)((cur.kvh << p.c.shift) + (key & ((1u << p.c.shift) - 1u)));
-                    unsigned int bad = __ballot_sync(0xFFFFFFFFu, lane < boxes && none);
+                    const unsigned int bad = __ballot_sync(0xFFFFFFFFu, lane < boxes && none);
                     if (i + 1 < units) { next = page_of(i + 1); }
-                    ok = tile < 2 || __all_sync(0xFFFFFFFFu, wait(k_empty + st, (tile >> 1) - 1));
+                    ok = n < NS || __all_sync(0xFFFFFFFFu, wait(k_empty + st, n / NS - 1));
                     if (!ok) { break; }
                     if (lane == 0)
                     {
                         unsigned int wide = 0;    // a bit for every sixteen keys
                         for (unsigned int b = 0; b < boxes; b++) { wide |= (bad >> b & 1u) ? ((1u << (box_rows / 16)) - 1u) << (b * (box_rows / 16)) : 0u; }
-                        bad_s[tile % INFOS] = wide;
-                        mbar_expect_tx(k_full + st, S::TILE);
+                        bad_s[n % INFOS] = wide;
+                        mbar_expect_tx(k_full + st, S::STAGE);
                     }
                     __syncwarp();
                     if (lane < boxes)
                     {
 #pragma unroll
-                        for (int b = 0; b < D / 64; b++) { tma_load_3d(ks + st * S::TILE + b * S::BLOCK + lane * box_rows * 128, &tmK, b * 64, row, z, k_full + st); }
+                        for (int b = 0; b < D / 64; b++) { tma_load_3d(ks + st * S::STAGE + b * S::BLOCK + lane * box_rows * 128, &tmK, b * 64, row, z, k_full + st); }
                     }
                     __syncwarp();
                     if (lane == 0) { mbar_arrive(k_full + st); }
-                    ok = tile < 2 || __all_sync(0xFFFFFFFFu, wait(v_empty + st, (tile >> 1) - 1));
+                    ok = n < NS || __all_sync(0xFFFFFFFFu, wait(v_empty + st, n / NS - 1));
                     if (!ok) { break; }
-                    if (lane == 0) { mbar_expect_tx(v_full + st, S::TILE); }
+                    if (lane == 0) { mbar_expect_tx(v_full + st, S::STAGE); }
                     __syncwarp();
                     if (lane < boxes)
                     {
 #pragma unroll
-                        for (int b = 0; b < D / 64; b++) { tma_load_3d(vs + st * S::TILE + b * S::BLOCK + lane * box_rows * 128, &tmV, b * 64, row, z, v_full + st); }
+                        for (int b = 0; b < D / 64; b++) { tma_load_3d(vs + st * S::STAGE + b * S::BLOCK + lane * box_rows * 128, &tmV, b * 64, row, z, v_full + st); }
                     }
                     __syncwarp();
                     if (lane == 0) { mbar_arrive(v_full + st); }
                 }
-                at += units;
+                at += units / HALVES;
                 if (at < length) { cur.next(p); }
             }
-            if (!ok && lane == 0) { give_up(0, tile); }
+            if (!ok && lane == 0) { give_up(0, n); }
             // the copies in flight arrive (bounded) before the CTA may leave
             if (lane == 0)
             {
-                for (unsigned int j = tile < 2 ? 0 : tile - 2; j < tile; j++)
+                for (unsigned int j = n < NS ? 0 : n - NS; j < n; j++)
                 {
-                    mbar_wait_bounded(k_full + (j & 1u), (j >> 1) & 1u);
-                    mbar_wait_bounded(v_full + (j & 1u), (j >> 1) & 1u);
+                    mbar_wait_bounded(k_full + j % NS, (j / NS) & 1u);
+                    mbar_wait_bounded(v_full + j % NS, (j / NS) & 1u);
                 }
-                if (!ok && tile >= 2) { mbar_wait_bounded(k_full + (tile & 1u), (tile >> 1) & 1u); }
+                if (!ok && n >= NS) { mbar_wait_bounded(k_full + n % NS, (n / NS) & 1u); }
             }
         }
         else
         {
-            // LPR lanes a row, sixteen codes each; the warps take a tile's groups of PER rows in turn, keys and then values (with them from where
-            // the keys have left off).  The next tile's rows are under way while this one's are turned into numbers.
-            constexpr unsigned int LPR = D / 16, PER = 32 / LPR, GROUPS = KT / PER, MOST = (GROUPS + S::LOADERS - 1) / S::LOADERS;
-            const unsigned int c = lane % LPR, r = lane / LPR, w = warp - LOAD;
-            const unsigned int first[2] = { w, (w + S::LOADERS - GROUPS % S::LOADERS) % S::LOADERS };
+            // LPR lanes a row, sixteen codes each; the warps take a stage's groups of PER rows in turn.  The next stage's rows are under way while this
+            // one's are turned into numbers, and the pages of the one behind that.
+            constexpr unsigned int LPR = D / 16, PER = 32 / LPR, GROUPS = 64 / PER, MOST = (GROUPS + S::LOADERS - 1) / S::LOADERS;
+            const unsigned int c = lane % LPR, r = lane / LPR, w = warp - LOAD, all = length * HALVES;
             uint4 raw[2][MOST];
             unsigned int two[2][MOST];
-            int sixteen = 0;    // the page of the lane's sixteen keys of the tile
-            unsigned int i = 0, at = 0, units = cur.take(length);    // the tile that is fetched next: of its segment; where that begins in the share
-            auto fetch = [&](int which) {
-                const unsigned int key0 = cur.s.unit(cur.unit + i) * KT, ld = which ? p.c.v_ld : p.c.k_ld;
-                const unsigned char *x = which ? p.c.v : p.c.k, *scale = which ? p.c.v_scale : p.c.k_scale;
+            // a stage's first key, kv head and pages: of the lane's rows, and of its sixteen keys
+            struct Place
+            {
+                unsigned int key0, kvh;
+                int page[MOST], sixteen;
+            } place = {};
+            unsigned int i = 0, at = 0, units = cur.take(length) * HALVES;    // the stage that is looked up next: of its segment; where that begins in the share
+            auto look_up = [&]() {
+                if (at >= length) { return; }
                 const int* table = p.c.table + (size_t)(unsigned int)cur.v.slot * p.c.ld_table;    // (looked at for a wanted key only)
-                int page[MOST];
+                place.key0 = cur.s.unit(cur.unit + i / HALVES) * KT + i % HALVES * 64;
+                place.kvh = cur.kvh;
 #pragma unroll
                 for (unsigned int a = 0; a < MOST; a++)
                 {
-                    const unsigned int group = first[which] + a * S::LOADERS, key = key0 + group * PER + r;
-                    page[a] = group < GROUPS && paged_wanted(cur.v, cur.s, key) ? table[key >> p.c.shift] : -1;
+                    const unsigned int group = w + a * S::LOADERS, key = place.key0 + group * PER + r;
+                    place.page[a] = group < GROUPS && paged_wanted(cur.v, cur.s, key) ? table[key >> p.c.shift] : -1;
                 }
-                if (which == 0)
+                const unsigned int key = place.key0 + lane * 16;
+                const bool meets = lane < 4 && key < cur.s.lim && (key + 16 > cur.s.low || (key + 16 > cur.v.floor && key < cur.s.first_end));
+                place.sixteen = meets ? table[key >> p.c.shift] : 0;
+                if (++i == units)
                 {
-                    const unsigned int key = key0 + lane * 16;
-                    const bool meets = lane < KT / 16 && key < cur.s.lim && (key + 16 > cur.s.low || (key + 16 > cur.v.floor && key < cur.s.first_end));
-                    sixteen = meets ? table[key >> p.c.shift] : 0;
+                    at += units / HALVES;
+                    i = 0;
+                    if (at < length)
+                    {
+                        cur.next(p);
+                        units = cur.take(length - at) * HALVES;
+                    }
                 }
+            };
+            auto fetch = [&](int which) {
+                const unsigned int ld = which ? p.c.v_ld : p.c.k_ld;
+                const unsigned char *x = which ? p.c.v : p.c.k, *scale = which ? p.c.v_scale : p.c.k_scale;
 #pragma unroll
                 for (unsigned int a = 0; a < MOST; a++)
                 {
-                    const unsigned int key = key0 + (first[which] + a * S::LOADERS) * PER + r;
-                    const bool have = (unsigned int)page[a] < p.c.pages;
-                    const size_t row = have ? paged_row(p.c, page[a], cur.kvh, key) : 0;
+                    const bool have = (unsigned int)place.page[a] < p.c.pages;
+                    const size_t row = have ? paged_row(p.c, place.page[a], place.kvh, place.key0 + (w + a * S::LOADERS) * PER + r) : 0;
                     raw[which][a] = have && c * 16 < ld ? *reinterpret_cast<const uint4*>(x + row * ld + c * 16) : make_uint4(0, 0, 0, 0);
                     two[which][a] = have ? scale[row] : 0u;
                 }
@@ -238,7 +243,7 @@ __global__ void __launch_bounds__(32 * TileShape<D, CODED>::WARPS, 1) paged_tile
 #pragma unroll
                 for (unsigned int a = 0; a < MOST; a++)
                 {
-                    const unsigned int group = first[which] + a * S::LOADERS, row = group * PER + r;
+                    const unsigned int group = w + a * S::LOADERS, row = group * PER + r;
                     if (group >= GROUPS) { break; }
                     const float f = paged_two(two[which][a]);
                     const uint4 u = raw[which][a];
@@ -252,138 +257,132 @@ __global__ void __launch_bounds__(32 * TileShape<D, CODED>::WARPS, 1) paged_tile
                 fence_proxy_async();
                 __syncwarp();
             };
+            look_up();
             fetch(0);
-            for (; tile < length && ok; tile++)
+            fetch(1);
+            unsigned int bad = __ballot_sync(0xFFFFFFFFu, (unsigned int)place.sixteen >= p.c.pages);
+            look_up();
+            for (; n < all; n++)
             {
-                const unsigned int st = tile & 1u;
-                fetch(1);
-                ok = tile < 2 || __all_sync(0xFFFFFFFFu, wait(k_empty + st, (tile >> 1) - 1));
+                const unsigned int st = n % NS;
+                ok = n < NS || __all_sync(0xFFFFFFFFu, wait(k_empty + st, n / NS - 1));
                 if (!ok) { break; }
-                const unsigned int bad = __ballot_sync(0xFFFFFFFFu, (unsigned int)sixteen >= p.c.pages);
-                if (w == 0 && lane == 0) { bad_s[tile % INFOS] = bad; }
-                store(0, ks + st * S::TILE);
+                if (w == 0 && lane == 0) { bad_s[n % INFOS] = bad; }
+                store(0, ks + st * S::STAGE);
                 if (lane == 0) { mbar_arrive(k_full + st); }
-                if (++i == units)
-                {
-                    at += units;
-                    i = 0;
-                    if (at < length)
-                    {
-                        cur.next(p);
-                        units = cur.take(length - at);
-                    }
-                }
-                if (tile + 1 < length) { fetch(0); }
-                ok = tile < 2 || __all_sync(0xFFFFFFFFu, wait(v_empty + st, (tile >> 1) - 1));
+                if (n + 1 < all) { fetch(0); }
+                ok = n < NS || __all_sync(0xFFFFFFFFu, wait(v_empty + st, n / NS - 1));
                 if (!ok) { break; }
-                store(1, vs + st * S::TILE);
+                store(1, vs + st * S::STAGE);
                 if (lane == 0) { mbar_arrive(v_full + st); }
+                if (n + 1 < all)
+                {
+                    fetch(1);
+                    bad = __ballot_sync(0xFFFFFFFFu, (unsigned int)place.sixteen >= p.c.pages);
+                }
+                look_up();
             }
-            if (!ok && lane == 0) { give_up(0, tile); }
+            if (!ok && lane == 0) { give_up(0, n); }
         }
     }
-    else if (warp == MMA)
+    else if (warp >= MMA)
     {
         const uint32_t idesc_s = umma_idesc_bf16(128, 64), idesc_o = umma_idesc_bf16(128, D) | (1u << 16);    // V is MN-major
         // (adding n >> 4 to a descriptor moves it on by n bytes)
-        const uint64_t q_desc = umma_desc_kmajor_sw128(smem_u32(qs)), k_desc = umma_desc_kmajor_sw128(smem_u32(ks)), v_desc = umma_desc_values(smem_u32(vs), S::BLOCK);
-        unsigned int tile = 0, queries[RT] = {}, weights[RT] = {};    // tiles taken; of each half of the rows: segments, tiles whose weights were waited for
+        const uint64_t q_desc = umma_desc_kmajor_sw128(smem_u32(qs)), k_desc = umma_desc_kmajor_sw128(smem_u32(ks)), v_desc = umma_desc_mnmajor_sw128(smem_u32(vs));
+        const unsigned int x = warp - MMA;              // the half of the rows whose products it issues
+        unsigned int n = 0, tile = 0, queries = 0;      // stages, and of this half tiles and segments
         bool ok = true;
+        // sixty-four keys, stage j, against the rows
+        auto scores = [&](unsigned int j, unsigned int h) {
+            if (!wait(k_full + j % NS, j / NS)) { return false; }
+            tc_fence_after();
+            if (elect_one())
+            {
+                const uint64_t q = q_desc + x * (D / 64) * (S::QBLOCK >> 4), kd = k_desc + j % NS * (S::STAGE >> 4);
+                const uint32_t to = tmem + x * S::S_COLS + h * 64;
+#pragma unroll
+                for (int k = 0; k < D / 16; k++)
+                {
+                    if (k * 16 < (int)p.c.dim)
+                    {
+                        umma_bf16(to, q + (k / 4) * (S::QBLOCK >> 4) + (k % 4) * 2, kd + (k / 4) * (S::BLOCK >> 4) + (k % 4) * 2, idesc_s, k != 0 ? 1u : 0u);
+                    }
+                }
+                umma_commit(k_empty + j % NS);
+                umma_commit(&s_full[x][h]);
+            }
+            __syncwarp();
+            return true;
+        };
         for (unsigned int at = 0; at < length && ok;)
         {
-            const unsigned int units = cur.take(length - at), halves = cur.s.rows > 128 ? RT : 1;
-            // sixty-four keys of tile j against one half of the rows
-            auto scores = [&](unsigned int x, unsigned int j, unsigned int h) {
-                if (elect_one())
+            const unsigned int units = cur.take(length - at);
+            if (x != 0 && cur.s.rows <= 128)
+            {
+                // not its segment: the stages are given back as they come
+                for (unsigned int i = 0; i < units * HALVES && ok; i++, n++)
                 {
-                    const uint64_t q = q_desc + x * (D / 64) * (S::QBLOCK >> 4), kd = k_desc + (j & 1u) * (S::TILE >> 4) + h * (64 * 128 >> 4);
-                    const uint32_t to = tmem + x * S::S_COLS + h * 64;
-#pragma unroll
-                    for (int k = 0; k < D / 16; k++)
+                    ok = wait(k_full + n % NS, n / NS) && wait(v_full + n % NS, n / NS);
+                    if (ok && lane == 0)
                     {
-                        if (k * 16 < (int)p.c.dim)
-                        {
-                            umma_bf16(to, q + (k / 4) * (S::QBLOCK >> 4) + (k % 4) * 2, kd + (k / 4) * (S::BLOCK >> 4) + (k % 4) * 2, idesc_s, k != 0 ? 1u : 0u);
-                        }
+                        mbar_arrive(k_empty + n % NS);
+                        mbar_arrive(v_empty + n % NS);
                     }
-                    if (x + 1 == halves && h + 1 == S::HALVES) { umma_commit(k_empty + (j & 1u)); }
-                    umma_commit(&s_full[x][h]);
+                    __syncwarp();
                 }
-                __syncwarp();
-            };
-            ok = wait(k_full + (tile & 1u), tile >> 1);
-#pragma unroll
-            for (unsigned int x = 0; x < RT; x++)
-            {
-                if (x >= halves || !ok) { break; }
-                ok = wait(q_ready + x, queries[x]++);
-                tc_fence_after();
-                for (unsigned int h = 0; ok && h < S::HALVES; h++) { scores(x, tile, h); }
             }
-            for (unsigned int i = 0; i < units && ok; i++, tile++)
+            else
             {
-                const unsigned int st = tile & 1u;
-                ok = wait(v_full + st, tile >> 1);
-                if (!ok) { break; }
+                ok = wait(q_ready + x, queries++);
                 tc_fence_after();
-                if constexpr (!CODED)
+                for (unsigned int h = 0; h < HALVES && ok; h++) { ok = scores(n + h, h); }
+                for (unsigned int i = 0; i < units && ok; i++, tile++)
                 {
-                    const unsigned int key0 = cur.s.unit(cur.unit + i) * KT;
-                    if (key0 < cur.s.low || key0 + KT > cur.s.lim)
+#pragma unroll 1
+                    for (unsigned int h = 0; h < HALVES && ok; h++, n++)
                     {
-                        // rows that nobody sees may hold anything
-                        for (unsigned int j = lane; j < KT; j += 32)
+                        const unsigned int st = n % NS;
+                        ok = wait(v_full + st, n / NS);
+                        if (!ok) { break; }
+                        if constexpr (!CODED)
                         {
-                            if (paged_wanted(cur.v, cur.s, key0 + j)) { continue; }
-#pragma unroll
-                            for (int b = 0; b < D / 64; b++)
+                            const unsigned int key0 = cur.s.unit(cur.unit + i) * KT + h * 64;
+                            if (key0 < cur.s.low || key0 + 64 > cur.s.lim)
                             {
+                                // rows that nobody sees may hold anything (both issuing warps clear them: each before its own product)
+                                for (unsigned int j = lane; j < 64; j += 32)
+                                {
+                                    if (paged_wanted(cur.v, cur.s, key0 + j)) { continue; }
 #pragma unroll
-                                for (int k = 0; k < 8; k++) { sts128(smem_u32(vs) + st * S::TILE + b * S::BLOCK + j * 128 + k * 16, 0, 0, 0, 0); }
+                                    for (int b = 0; b < D / 64; b++)
+                                    {
+#pragma unroll
+                                        for (int k = 0; k < 8; k++) { sts128(smem_u32(vs) + st * S::STAGE + b * S::BLOCK + j * 128 + k * 16, 0, 0, 0, 0); }
+                                    }
+                                }
+                                fence_proxy_async();
+                                __syncwarp();
                             }
                         }
-                        fence_proxy_async();
-                        __syncwarp();
-                    }
-                }
-#pragma unroll 1
-                for (unsigned int h = 0; h < S::HALVES; h++)
-                {
-#pragma unroll
-                    for (unsigned int x = 0; x < RT; x++)
-                    {
-                        if (x >= halves || !ok) { break; }
-                        ok = wait(&p_ready[x][h], weights[x]);
+                        ok = wait(&p_ready[x][h], tile);
                         if (!ok) { break; }
                         tc_fence_after();
                         if (elect_one())
                         {
-                            const uint64_t vd = v_desc + st * (S::TILE >> 4) + h * (4 * 2048 >> 4);
+                            const uint64_t vd = v_desc + st * (S::STAGE >> 4);
 #pragma unroll
                             for (int k = 0; k < 4; k++)
                             {
                                 umma_bf16_ts(tmem + S::O_AT + x * D, tmem + x * S::S_COLS + h * 64 + k * 8, vd + k * (2048 >> 4), idesc_o, (i | h | (unsigned int)k) != 0 ? 1u : 0u);
                             }
                             umma_commit(pv_done + x);
-                            if (h + 1 == S::HALVES)
-                            {
-                                if (x + 1 == halves) { umma_commit(v_empty + st); }
-                                if (i + 1 == units) { umma_commit(o_full + x); }
-                            }
+                            umma_commit(v_empty + st);
+                            if (h + 1 == HALVES && i + 1 == units) { umma_commit(o_full + x); }
                         }
                         __syncwarp();
-                        if (h + 1 == S::HALVES) { weights[x]++; }
                         // into the place of the weights just issued: products of one thread run in the order of their issue
-                        if (i + 1 < units)
-                        {
-                            if (x == 0 && h == 0)
-                            {
-                                ok = wait(k_full + ((tile + 1) & 1u), (tile + 1) >> 1);
-                                if (!ok) { break; }
-                                tc_fence_after();
-                            }
-                            scores(x, tile + 1, h);
-                        }
+                        if (i + 1 < units) { ok = scores(n + HALVES, h); }
                     }
                 }
             }
@@ -392,8 +391,8 @@ __global__ void __launch_bounds__(32 * TileShape<D, CODED>::WARPS, 1) paged_tile
         }
         if (!ok)
         {
-            if (lane == 0) { give_up(1, tile); }
-            if (elect_one()) { umma_commit(pv_done); }    // completes once the products in flight have stopped reading shared memory
+            if (lane == 0) { give_up(1, n); }
+            if (elect_one()) { umma_commit(pv_done + x); }    // completes once the products in flight have stopped reading shared memory
             __syncwarp();
         }
     }
@@ -419,23 +418,39 @@ __global__ void __launch_bounds__(32 * TileShape<D, CODED>::WARPS, 1) paged_tile
             const unsigned int t = v.pos + (real ? r / p.G : 0), tok = v.start + (real ? r / p.G : 0), head = cur.kvh * p.G + (real ? r % p.G : 0);
             if (active)
             {
-                const __nv_bfloat16* src = (const __nv_bfloat16*)p.q + (size_t)tok * p.ldq + (size_t)head * p.c.dim;
-#pragma unroll 16
-                for (int c = 0; c < D / 8; c++)
+                const size_t from = (size_t)tok * p.ldq + (size_t)head * p.c.dim;
+                const uint32_t place_q = smem_u32(qs) + x * (D / 64) * S::QBLOCK + quarter * 32 * 128;    // of the warp's rows
+                if (vec_q)
                 {
-                    uint4 u = make_uint4(0, 0, 0, 0);
-                    if (real && c * 8 < (int)p.c.dim)
-                    {
-                        if (vec_q) { u = *reinterpret_cast<const uint4*>(src + c * 8); }
-                        else
-                        {
-                            uint32_t w[8];
+                    // a row by neighbouring lanes: whole lines, all of them under way at once
+                    constexpr unsigned int CH = D / 8, EACH = 32 / CH;
+                    uint4 u[CH];
 #pragma unroll
-                            for (int j = 0; j < 8; j++) { w[j] = c * 8 + j < (int)p.c.dim ? __bfloat16_as_ushort(src[c * 8 + j]) : 0u; }
-                            u = make_uint4(w[0] | (w[1] << 16), w[2] | (w[3] << 16), w[4] | (w[5] << 16), w[6] | (w[7] << 16));
-                        }
+                    for (unsigned int j = 0; j < CH; j++)
+                    {
+                        const unsigned int row = j * EACH + lane / CH, c = lane % CH;
+                        const size_t off = __shfl_sync(0xFFFFFFFFu, (unsigned long long)from, row);
+                        u[j] = x * 128 + quarter * 32 + row < s.rows && c * 8 < p.c.dim ? *reinterpret_cast<const uint4*>((const __nv_bfloat16*)p.q + off + c * 8)
+                                                                                        : make_uint4(0, 0, 0, 0);
                     }
-                    sts128(smem_u32(qs) + (x * (D / 64) + c / 8) * S::QBLOCK + rl * 128 + (((c % 8) ^ (rl & 7u)) * 16), u.x ^ flip, u.y ^ flip, u.z ^ flip, u.w ^ flip);
+#pragma unroll
+                    for (unsigned int j = 0; j < CH; j++)
+                    {
+                        const unsigned int row = j * EACH + lane / CH, c = lane % CH;
+                        sts128(place_q + (c / 8) * S::QBLOCK + row * 128 + (((c % 8) ^ (row & 7u)) * 16), u[j].x ^ flip, u[j].y ^ flip, u[j].z ^ flip, u[j].w ^ flip);
+                    }
+                }
+                else
+                {
+                    const __nv_bfloat16* src = (const __nv_bfloat16*)p.q + from;
+                    for (int c = 0; c < D / 8; c++)
+                    {
+                        uint32_t w[8];
+#pragma unroll
+                        for (int j = 0; j < 8; j++) { w[j] = real && c * 8 + j < (int)p.c.dim ? __bfloat16_as_ushort(src[c * 8 + j]) : 0u; }
+                        sts128(place_q + (c / 8) * S::QBLOCK + lane * 128 + (((c % 8) ^ (lane & 7u)) * 16), (w[0] | (w[1] << 16)) ^ flip, (w[2] | (w[3] << 16)) ^ flip,
+                            (w[4] | (w[5] << 16)) ^ flip, (w[6] | (w[7] << 16)) ^ flip);
+                    }
                 }
                 fence_proxy_async();
                 tc_fence_before();    // the last segment's outputs have been read before this one's products
@@ -453,7 +468,7 @@ __global__ void __launch_bounds__(32 * TileShape<D, CODED>::WARPS, 1) paged_tile
                 {
                     const unsigned int key0 = s.unit(cur.unit + i) * KT;
 #pragma unroll
-                    for (int h = 0; h < S::HALVES; h++)
+                    for (int h = 0; h < HALVES; h++)
                     {
                         ok = __all_sync(0xFFFFFFFFu, wait(&s_full[x][h], scored));
                         if (!ok) { break; }
@@ -462,7 +477,7 @@ __global__ void __launch_bounds__(32 * TileShape<D, CODED>::WARPS, 1) paged_tile
                         tmem_ld_32x32(place + h * 64, *reinterpret_cast<uint32_t(*)[32]>(z));
                         tmem_ld_32x32(place + h * 64 + 32, *reinterpret_cast<uint32_t(*)[32]>(z + 32));
                         tmem_ld_wait();
-                        const unsigned int k0 = key0 + h * 64, bad = bad_s[(tile + i) % INFOS] >> (h * 4) & 15u;
+                        const unsigned int k0 = key0 + h * 64, bad = bad_s[((tile + i) * HALVES + h) % INFOS];
                         if (bad != 0 || k0 < low_all || k0 + 64 > lim_all)
                         {
                             // the keys that the row sees, a bit each
@@ -474,9 +489,9 @@ __global__ void __launch_bounds__(32 * TileShape<D, CODED>::WARPS, 1) paged_tile
 #pragma unroll
                             for (int j = 0; j < 64; j++) { z[j] = (w[j / 32] >> (j % 32) & 1u) != 0 ? z[j] : 0xFF800000u; }    // else -inf
                         }
-                        float mx[4] = { -INFINITY, -INFINITY, -INFINITY, -INFINITY };    // four maxima in flight
+                        float mx[4] = { -INFINITY, -INFINITY, -INFINITY, -INFINITY };    // four maxima in flight, two numbers at a time
 #pragma unroll
-                        for (int j = 0; j < 64; j++) { mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(z[j])); }
+                        for (int j = 0; j < 32; j++) { mx[j & 3] = fmaxf(mx[j & 3], fmaxf(__uint_as_float(z[2 * j]), __uint_as_float(z[2 * j + 1]))); }
                         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale2;
                         float c = 1.f;
                         if (top > m + 8.f)
@@ -532,45 +547,49 @@ __global__ void __launch_bounds__(32 * TileShape<D, CODED>::WARPS, 1) paged_tile
                 const bool whole = cur.whole(units);
                 float* piece = p.partial + (2 * (size_t)blockIdx.x + (cur.unit == 0 ? 1 : 0)) * paged_piece(ROWS, p.c.vdim);
                 const float f = whole ? paged_factor(p, head, m, l) : 1.f;
-                __nv_bfloat16* out = (__nv_bfloat16*)p.out + (size_t)tok * p.ldo + (size_t)head * p.c.vdim;
-#pragma unroll
-                for (int d = 0; d < D; d += 32)
+                // by way of the queries' place (nothing reads it any more), so that neighbouring lanes write a row
+                const size_t to = (size_t)tok * p.ldo + (size_t)head * p.c.vdim;
+                const uint32_t stage = smem_u32(qs) + x * (D / 64) * S::QBLOCK + quarter * 32 * 128;
+                const unsigned int row0 = x * 128 + quarter * 32;
+#pragma unroll 1
+                for (int d = 0; d < (int)VL; d += 32)
                 {
-                    if (d >= (int)p.c.vdim) { break; }
                     uint32_t o[32];
                     tmem_ld_32x32(o_at + d, o);
                     tmem_ld_wait();
-                    if (real)
+                    if (!whole)
                     {
 #pragma unroll
-                        for (int q = 0; q < 32; q += 8)
-                        {
-                            float y[8];
+                        for (int q = 0; q < 8; q++) { sts128(stage + lane * 128 + ((q ^ (lane & 7u)) * 16), o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]); }
+                        __syncwarp();
 #pragma unroll
-                            for (int j = 0; j < 8; j++) { y[j] = __uint_as_float(o[q + j]) * f; }
-                            if (!whole)
-                            {
-                                if (d + q < (int)VL)
-                                {
-                                    store4(piece + (size_t)i_row * VL + d + q, make_float4(y[0], y[1], y[2], y[3]));
-                                    store4(piece + (size_t)i_row * VL + d + q + 4, make_float4(y[4], y[5], y[6], y[7]));
-                                }
-                            }
-                            else if (vec_o)
-                            {
-                                if (d + q < (int)p.c.vdim)
-                                {
-                                    *reinterpret_cast<uint4*>(out + d + q) =
-                                        make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]), pack_bf16x2(y[6], y[7]));
-                                }
-                            }
+                        for (unsigned int j = 0; j < 8; j++)
+                        {
+                            const unsigned int row = j * 4 + lane / 8, c = lane % 8;
+                            const uint4 u = lds128(stage + row * 128 + ((c ^ (row & 7u)) * 16));
+                            if (row0 + row < s.rows && d + c * 4 < VL) { *reinterpret_cast<uint4*>(piece + (size_t)(row0 + row) * VL + d + c * 4) = u; }
+                        }
+                    }
+                    else
+                    {
+                        uint32_t h[16];
+#pragma unroll
+                        for (int q = 0; q < 16; q++) { h[q] = pack_bf16x2(__uint_as_float(o[2 * q]) * f, __uint_as_float(o[2 * q + 1]) * f); }
+#pragma unroll
+                        for (int q = 0; q < 4; q++) { sts128(stage + lane * 128 + ((q ^ (lane & 7u)) * 16), h[4 * q], h[4 * q + 1], h[4 * q + 2], h[4 * q + 3]); }
+                        __syncwarp();
+#pragma unroll
+                        for (unsigned int j = 0; j < 4; j++)
+                        {
+                            const unsigned int row = j * 8 + lane / 4, c = lane % 4, at8 = d + c * 8;
+                            const uint4 u = lds128(stage + row * 128 + ((c ^ (row & 7u)) * 16));
+                            __nv_bfloat16* out = (__nv_bfloat16*)p.out + __shfl_sync(0xFFFFFFFFu, (unsigned long long)to, row) + at8;
+                            if (row0 + row >= s.rows || at8 >= p.c.vdim) { continue; }
+                            if (vec_o) { *reinterpret_cast<uint4*>(out) = u; }
                             else
                             {
-#pragma unroll
-                                for (int j = 0; j < 8; j++)
-                                {
-                                    if (d + q + j < (int)p.c.vdim) { out[d + q + j] = __float2bfloat16_rn(y[j]); }
-                                }
+                                const uint32_t w[4] = { u.x, u.y, u.z, u.w };
+                                for (unsigned int k = 0; k < 8 && at8 + k < p.c.vdim; k++) { out[k] = __ushort_as_bfloat16((unsigned short)(w[k / 2] >> (16 * (k % 2)))); }
                             }
                         }
                     }
@@ -605,7 +624,7 @@ static int run_tile(PagedParams& p, unsigned int sms, unsigned int* piece_rows, 
     *piece_rows = S::ROWS;
     unsigned int* status = decoder_status_word();
     if (!status) { return 1; }
-    const unsigned int page = 1u << p.c.shift, box = page < (unsigned int)S::KT ? page : (unsigned int)S::KT;
+    const unsigned int page = 1u << p.c.shift, box = page < 64 ? page : 64;
     CUtensorMap tk, tv;
     memset(&tk, 0, sizeof(tk));
     memset(&tv, 0, sizeof(tv));
