@@ -344,7 +344,15 @@ C_EXPORT int cuda_b200_paged_attention_rows(int dtype, const cuda_b200_paged_att
     const unsigned int rows = b->max_n * p.G, sms = (unsigned int)dev->sm_count;
     if (a->work_bytes < work_for(sms, rows, c->vdim)) { return -1; }
     if (dtype == DT_FLOAT) { kernel = 1; }
-    if (kernel == 0) { kernel = rows <= kPagedFewRows ? 2 : 3; }
+    if (kernel == 0)
+    {
+        // The kernel for few rows reads the cache once for every sixteen of them; the other one takes about as long for 20 as for 256, and where E4M3
+        // becomes BF16 before the products longer than its bytes.  us, few / many, 32 sequences of 4000 rows, 8 kv heads of 128:
+        // BF16 20 rows 194 / 141; E4M3 32 rows 128 / 339, 64 rows 209 / 344, 96 rows 300 / 350; one sequence of 30000 in E4M3 64 rows 64 / 92,
+        // 96 rows 91 / 92.  Heads of 64 and of 256 in E4M3: 20 rows 27 / 26, 45 / 35.
+        const unsigned int width = c->dim > c->vdim ? c->dim : c->vdim;
+        kernel = rows <= (coded && width > 64 && width <= 128 ? 4 * kPagedFewRows : kPagedFewRows) ? 2 : 3;
+    }
     if (kernel == 3 && a->work_bytes < work_of(sms, 1, 256, c->vdim)) { return -1; }
     if (kernel == 2)
     {

@@ -274,7 +274,7 @@ class Attention:
         each at most; on tcgen05 one BF16 number, so that sum |dw v| <= 2^-8 sum |w v|), on the sum of |weight * value|; and, on the same,
         what a score may be off: products and sums of dim terms in 32 bits, (dim + 8) * 2^-24 of the sum of |q k| * scale, twice
         (numerator and denominator), with as much again for the exponential (2^-22) and the sums of the keys' terms (keys * 2^-24)."""
-        many = kernel == MANY or (kernel == 0 and self.G * max(n for _, _, n in self.entries) > 16)
+        many = kernel == MANY or (kernel == 0 and self.G * max(n for _, _, n in self.entries) > 16)    # (where that is the one taken)
         weight = 0 if self.dtype == FLOAT else 2.0 ** -8 if many else 2.0 ** -10
         q = self.q.double().cpu().numpy()[:self.T].reshape(self.T, self.H, self.dim)
         out, tol, at = np.zeros((self.T, self.H, self.vdim)), np.zeros((self.T, self.H, self.vdim)), 0
