@@ -25,6 +25,14 @@ inline bool make_paged_map(CUtensorMap* map, bool coded, const void* base, unsig
         == CUDA_SUCCESS;
 }
 
+// Has the kernel been given this many registers a thread?  A split of them at run time that adds up to more would wait for good.
+template <class K>
+inline bool paged_registers(K kernel, int least)
+{
+    cudaFuncAttributes a;
+    return cudaFuncGetAttributes(&a, kernel) == cudaSuccess && a.numRegs >= least;
+}
+
 // The plain kernel: packed query rows of a segment, CTAs per SM.  The one for few rows (8 or 16 of them): warps of an SM that take shares.
 constexpr unsigned int kPagedPlainRows = 4, kPagedPlainCtas = 4, kPagedRowsWarps = 8;
 // Packed query rows of an entry up to which that one is taken.

@@ -11,8 +11,12 @@
 // E4M3: codes become FP16 by one instruction per pair, exactly.  Queries enter as FP16, each row by a power of two below 2^15
 // (exact for elements down to 2^-28 of the row's largest).  A key's power of two multiplies its score.  A value's one, 2^u, goes to the
 // weight: with m the maximum of score + u, p = 2^(score - m) counts in the sum and w = p 2^u <= 2^8 in the product, as FP16 - the
-// weights are rounded by 2^-12 of each at most, whatever the rows' scales.  BF16: weights enter as the sum of two BF16 numbers.
+// weights are rounded by 2^-11 of each at most (below 2^-14 by 2^-25), whatever the rows' scales.  BF16: weights enter as the sum of two BF16 numbers.
 // The maximum moves only when it grows by more than 2^8, so that the outputs are seldom rescaled.
+//
+// Measured: 32 sequences of 4096 rows in E4M3, 8 kv heads of 128 (271 MB), 56 us, 0.74 of the copy rate; 48 of up to 4000 in BF16, two tokens each (509 MB), 93,
+// 0.83.  In E4M3 some 600 instructions a warp for 8 KB are what is left (issue slots 40 % busy, ALU 40 %, 7.7 cycles an instruction); 4 us are the
+// launch and the search for the shares.
 #include "paged_attention.cuh"
 
 #include "../gemv_decode.cuh"
@@ -668,6 +672,9 @@ static int run_rows(PagedParams& p, unsigned int rows, unsigned int sms, unsigne
     CUtensorMap tk, tv;
     const unsigned int cols = (S::WIDE ? 128 : 64) / S::EB;
     if (!make_paged_map(&tk, CODED, p.c.k, p.c.k_ld, p.c, cols, 16, S::WIDE) || !make_paged_map(&tv, CODED, p.c.v, p.c.v_ld, p.c, cols, 16, S::WIDE)) { return -1; }
+    static const bool split[2] = { S::WARPS != 8 || paged_registers(paged_rows_kernel<D, CODED, 1>, S::lean(1) ? 96 : 128),
+        S::WARPS != 8 || paged_registers(paged_rows_kernel<D, CODED, 2>, S::lean(2) ? 96 : 128) };
+    if (!split[rows <= 8 ? 0 : 1]) { return -1; }
     const dim3 grid(sms), block(64 * S::WARPS);
     return rows <= 8 ? launch_kernel("paged_rows", paged_rows_kernel<D, CODED, 1>, grid, block, (size_t)S::SMEM, stream, pdl, tk, tv, p, status)
                      : launch_kernel("paged_rows", paged_rows_kernel<D, CODED, 2>, grid, block, (size_t)S::SMEM, stream, pdl, tk, tv, p, status);

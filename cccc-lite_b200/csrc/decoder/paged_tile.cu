@@ -8,11 +8,15 @@
 // The running maximum only moves when it grows by more than 2^8, so that O is seldom rescaled.
 //
 // BF16 pages come by TMA (128-byte swizzle); rows that no query of the segment sees are cleared before the value product, since
-// 0 times what is no number is none.  E4M3 pages come through registers: four warps turn codes into the BF16 numbers that they stand
-// for, power of two included - exact, four significant bits - so that everything behind is the same for both.
+// 0 times what is no number is none.  E4M3 pages come through registers: the warps that are left turn codes into the BF16 numbers that they
+// stand for, power of two included - exact, four significant bits - so that everything behind is the same for both.
 //
 // The weights are rounded to BF16 for the value product (2^-8 of each at most, half a step; their sum is kept in 32 bits): with the sum
 // of two BF16 numbers instead, the tensor cores have one and a half times the work.
+//
+// Measured, heads of 128, 32 on 8: 2048 tokens behind 8000 in BF16 306 us, 0.61 of the tensor cores' rate (1621 TFLOP/s); without the exponentials 282: the
+// products of 64 keys read both operands from shared memory at 1.3 times the time of 128, which would leave no second place for scores in
+// tensor memory (420 us).  The same in E4M3 551: loads through registers and the conversion; 407 with neither.
 //
 // Every wait is bounded; on expiry the status word is raised, the roles drain, tensor memory is freed and the CTA returns.
 #include "paged_attention.cuh"
@@ -32,7 +36,8 @@ struct TileShape
     static constexpr int ROWS = 128 * RT;
     static constexpr int LOADERS = CODED ? 8 - RT : 1;    // warps
     static constexpr int WARPS = 4 * RT + LOADERS + RT;   // a warpgroup and an issuing warp for each half of the rows
-    // E4M3 with two halves: 128 registers each at launch, then 136 for the two warpgroups of the rows and 120 for the others
+    // E4M3 with two halves: 128 registers each at launch, then more for the two warpgroups of the rows than for the others (heads of 128: 144 and 112, 551 us
+    // for 2048 tokens behind 8000; 136 and 120 602, 152 and 104 581.  Of 64: 136 and 120, 409; 144 and 112 433, 152 and 104 438)
     static constexpr bool SPLIT = CODED && RT == 2;
     static constexpr int QBLOCK = 128 * 128, BLOCK = 64 * 128;    // bytes of 64 elements of 128 query rows, of 64 keys
     static constexpr int Q_BYTES = RT * (D / 64) * QBLOCK;
@@ -44,13 +49,17 @@ struct TileShape
     static constexpr uint32_t COLS = RT * (KT + D) <= 256 ? 256 : 512;
 };
 
-// Four codes times their row's power of two, as BF16 (exact).
-__device__ __forceinline__ uint2 e4m3x4_to_bf16(uint32_t four, float two)
+// Four codes times their row's power of two (twice, as BF16), as BF16.  Exact: four significant bits are the upper halves of floats, and a power
+// of two leaves them as they are.
+__device__ __forceinline__ uint2 e4m3x4_to_bf16(uint32_t four, uint32_t two)
 {
     uint32_t a, b;
     e4m3x4_to_f16x2(four, a, b);
     const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&a)), y = __half22float2(*reinterpret_cast<const __half2*>(&b));
-    return make_uint2(pack_bf16x2(x.x * two, x.y * two), pack_bf16x2(y.x * two, y.y * two));
+    uint2 r = make_uint2(__byte_perm(__float_as_uint(x.x), __float_as_uint(x.y), 0x7632), __byte_perm(__float_as_uint(y.x), __float_as_uint(y.y), 0x7632));
+    asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(r.x) : "r"(two));
+    asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(r.y) : "r"(two));
+    return r;
 }
 
 template <int D, bool CODED>
@@ -113,8 +122,16 @@ __global__ void __launch_bounds__(32 * TileShape<D, CODED>::WARPS, 1) paged_tile
 
     if constexpr (S::SPLIT)
     {
-        if (warp < LOAD) { asm volatile("setmaxnreg.inc.sync.aligned.u32 136;"); }
-        else { asm volatile("setmaxnreg.dec.sync.aligned.u32 120;"); }
+        if (warp < LOAD)
+        {
+            if constexpr (D == 128) { asm volatile("setmaxnreg.inc.sync.aligned.u32 144;"); }
+            else { asm volatile("setmaxnreg.inc.sync.aligned.u32 136;"); }
+        }
+        else
+        {
+            if constexpr (D == 128) { asm volatile("setmaxnreg.dec.sync.aligned.u32 112;"); }
+            else { asm volatile("setmaxnreg.dec.sync.aligned.u32 120;"); }
+        }
     }
     if (length == 0) {}
     else if (warp >= LOAD && warp < MMA)
@@ -189,7 +206,7 @@ __global__ void __launch_bounds__(32 * TileShape<D, CODED>::WARPS, 1) paged_tile
         }
         else
         {
-            // LPR lanes a row, sixteen codes each; the warps take a stage's groups of PER rows in turn.  The next stage's rows are under way while this
+            // LPR lanes a row, eight codes of its first and of its second half each (so that no two lanes meet in a bank of the stage); the warps take a stage's groups of PER rows in turn.  The next stage's rows are under way while this
             // one's are turned into numbers, and the pages of the one behind that.
             constexpr unsigned int LPR = D / 16, PER = 32 / LPR, GROUPS = 64 / PER, MOST = (GROUPS + S::LOADERS - 1) / S::LOADERS;
             const unsigned int c = lane % LPR, r = lane / LPR, w = warp - LOAD, all = length * HALVES;
@@ -235,7 +252,10 @@ __global__ void __launch_bounds__(32 * TileShape<D, CODED>::WARPS, 1) paged_tile
                 {
                     const bool have = (unsigned int)place.page[a] < p.c.pages;
                     const size_t row = have ? paged_row(p.c, place.page[a], place.kvh, place.key0 + (w + a * S::LOADERS) * PER + r) : 0;
-                    raw[which][a] = have && c * 16 < ld ? *reinterpret_cast<const uint4*>(x + row * ld + c * 16) : make_uint4(0, 0, 0, 0);
+                    const unsigned char* from = x + row * ld + c * 8;
+                    const uint2 lo = have && c * 8 < ld ? *reinterpret_cast<const uint2*>(from) : make_uint2(0, 0);
+                    const uint2 hi = have && D / 2 + c * 8 < ld ? *reinterpret_cast<const uint2*>(from + D / 2) : make_uint2(0, 0);
+                    raw[which][a] = make_uint4(lo.x, lo.y, hi.x, hi.y);
                     two[which][a] = have ? scale[row] : 0u;
                 }
             };
@@ -245,14 +265,13 @@ __global__ void __launch_bounds__(32 * TileShape<D, CODED>::WARPS, 1) paged_tile
                 {
                     const unsigned int group = w + a * S::LOADERS, row = group * PER + r;
                     if (group >= GROUPS) { break; }
-                    const float f = paged_two(two[which][a]);
+                    const uint32_t f = two[which][a] * 0x00800080u;    // the exponent, twice
                     const uint4 u = raw[which][a];
                     const uint2 x0 = e4m3x4_to_bf16(u.x, f), x1 = e4m3x4_to_bf16(u.y, f), x2 = e4m3x4_to_bf16(u.z, f), x3 = e4m3x4_to_bf16(u.w, f);
-                    const uint32_t base = smem_u32(to) + (c / 4) * S::BLOCK + row * 128, p0 = (((c % 4) * 2) ^ (row & 7u)) * 16, p1 = p0 ^ 16;
-                    // the lanes of every other block begin with their second piece: no two meet in a bank
-                    const bool turn = ((c / 4) & 1u) != 0;
-                    sts128(base + (turn ? p1 : p0), turn ? x2.x : x0.x, turn ? x2.y : x0.y, turn ? x3.x : x1.x, turn ? x3.y : x1.y);
-                    sts128(base + (turn ? p0 : p1), turn ? x0.x : x2.x, turn ? x0.y : x2.y, turn ? x1.x : x3.x, turn ? x1.y : x3.y);
+                    const uint32_t base = smem_u32(to) + row * 128;
+                    auto piece = [&](unsigned int code) { return base + code / 64 * S::BLOCK + ((code % 64 / 8 ^ (row & 7u)) * 16); };
+                    sts128(piece(c * 8), x0.x, x0.y, x1.x, x1.y);
+                    sts128(piece(D / 2 + c * 8), x2.x, x2.y, x3.x, x3.y);
                 }
                 fence_proxy_async();
                 __syncwarp();
@@ -624,6 +643,8 @@ static int run_tile(PagedParams& p, unsigned int sms, unsigned int* piece_rows, 
     *piece_rows = S::ROWS;
     unsigned int* status = decoder_status_word();
     if (!status) { return 1; }
+    static const bool split = !S::SPLIT || paged_registers(paged_tile_kernel<D, CODED>, 128);
+    if (!split) { return -1; }
     const unsigned int page = 1u << p.c.shift, box = page < 64 ? page : 64;
     CUtensorMap tk, tv;
     memset(&tk, 0, sizeof(tk));

@@ -440,6 +440,28 @@ def test_scores_of_minus_infinity(D):
         assert np.all(np.abs(got[1] - want_all[1]) <= 2.0 ** -7 * np.abs(want_all[1]) + 2.0 ** -9) and np.all(np.isfinite(got)) and k.shape[0] == 71
 
 
+@pytest.mark.parametrize("dtype,type_", TYPES[:3])
+@pytest.mark.parametrize("scale", [-0.3, 1e-30])
+def test_scales_below_and_next_to_zero(D, dtype, type_, scale):
+    a = Attention(D, dtype, type_, 8, 2, 64, 64, [(0, 130, 1), (1, 60, 25)], scale=scale, sink=True, seed=14)
+    a.sink[3] = -np.inf    # a sink that takes nothing
+    for kernel in kinds(dtype, 8, 2, a.entries):
+        a.check(kernel, scale)
+
+
+@pytest.mark.parametrize("dtype,type_", TYPES[:3])
+def test_a_query_that_is_no_number_spoils_its_own_rows(D, dtype, type_):
+    a = Attention(D, dtype, type_, 8, 2, 64, 64, [(0, 130, 1), (1, 60, 25)], seed=15)
+    want, _ = a.reference()
+    a.q[4, 2 * 64 + 5] = float("nan")
+    for kernel in kinds(dtype, 8, 2, a.entries):
+        got = a.run(kernel)
+        none = np.isnan(got)
+        assert np.all(none[4, 2]) and none.sum() == 64
+        tol = np.nan_to_num(a.reference(kernel=kernel)[1], nan=1.0)
+        assert np.all(np.abs(got - want)[~none] <= tol[~none]), kernel
+
+
 @pytest.mark.parametrize("type_", [BF16, E4M3])
 def test_one_long_sequence(D, type_):
     """Shares of every CTA in one segment."""
