@@ -639,7 +639,7 @@ template <int D, bool CODED>
 static int run_tile(PagedParams& p, unsigned int sms, unsigned int* piece_rows, cudaStream_t stream, bool pdl)
 {
     using S = TileShape<D, CODED>;
-    p.least = 2;
+    p.least = 1;    // (two tiles at least: a prompt of 128 tokens 26 us instead of 17, of 300 34 instead of 26, of 512 the same)
     *piece_rows = S::ROWS;
     unsigned int* status = decoder_status_word();
     if (!status) { return 1; }
