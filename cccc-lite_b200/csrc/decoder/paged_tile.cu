@@ -103,11 +103,11 @@ __global__ void __launch_bounds__(32 * TileShape<D, CODED>::WARPS, 1) paged_tile
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == MMA) { tmem_alloc(&tmem_slot, S::COLS); }
-    grid_dependency_launch();
     grid_dependency_wait();
     tc_fence_before();
     paged_sums<KT, ROWS, THREADS>(p, &sums);    // (its barriers stand behind what is set up above)
     tc_fence_after();
+    grid_dependency_launch();    // only now that this CTA has its tensor memory: a kernel behind it that took that first would wait for this one for good
     const uint32_t tmem = tmem_slot;
     const PagedShare share = paged_share<KT, ROWS, THREADS>(p, sums, blockIdx.x, gridDim.x);
     const unsigned int length = (unsigned int)(share.end - share.begin);

@@ -671,3 +671,22 @@ def test_a_graph_whose_sequences_grow(D):
         got = out.double().cpu().numpy().reshape(2, H, dim)
         assert np.all(np.abs(got - want) <= tol), i
         assert np.all(np.abs(oo.double().cpu().numpy().reshape(other.T, 4, 128) - other_want) <= other_tol), i
+
+
+def test_prompts_one_behind_the_other(D):
+    """Many calls for many query rows in a row, each allowed to start before the one in front has ended: two of them fit an SM, tensor memory for one."""
+    import torch
+
+    a = Attention(D, BF16, BF16, 8, 2, 64, 64, [(0, 0, 200), (1, 300, 90)], seed=16)
+    want, tol = a.reference()
+    b, keep = batch(D, a.entries)
+    pages = a.c.fill()
+    outs = [torch.zeros(a.T, 8 * 64, dtype=torch.bfloat16, device="cuda") for _ in range(6)]
+    work = torch.zeros(D.paged_attention_work_bytes(8, 2, 64, 200), dtype=torch.uint8, device="cuda")
+    descs = [D.fill(D.PagedAttention, q=a.q, out=o, work=work, work_bytes=work.numel(), ldq=512, ldo=512, H=8, scale=a.scale) for o in outs]
+    for _ in range(5):
+        for d in descs:
+            assert D.paged_attention(BF16, d, pages, b, flags=1) == 0
+    assert D.check() == 0
+    for o in outs:
+        assert np.all(np.abs(o.double().cpu().numpy().reshape(want.shape) - want) <= tol)
